@@ -2088,3 +2088,242 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
         check(lib.lse_delta_scan(*inputs, segments, heads, groups, dim, vdim, state.shape[0], above if chunked else 0, _stream()),
               "delta_scan")
     return out
+
+
+# ------------------------------------------------------------------ keys and values in 4 bits
+# A row of D values of a head is held as codes u in 0 .. 15 (uint8 [pages, n_kv, page_size, D / 2], byte b: d = 2 b low, 2 b + 1 high)
+# with a scale s and a centre c (bfloat16 [pages, n_kv, page_size, 2]) and stands for s (u - 8) + c.
+def _want(name: str, ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(f"{name}: {what}")
+
+
+def _here(name: str, *tensors: torch.Tensor) -> None:
+    """CUDA tensors of the current device: a kernel is launched on that one's stream."""
+    _need_cuda(*tensors)
+    device = torch._C._cuda_getDevice()
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != device:
+            raise KernelError(f"{name}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
+
+
+def _int4_pages(name: str, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+    """(pages, key/value heads, page size, head size) of a 4-bit cache's four tensors."""
+    _want(name, k_codes.dim() == 4 and k_codes.dtype == torch.uint8 and v_codes.dtype == torch.uint8 and v_codes.shape == k_codes.shape,
+          "codes are uint8 [pages, key/value heads, page size, head size / 2]")
+    pages, n_kv, page_size, half = k_codes.shape
+    _want(name, half in (32, 64), f"head size {2 * half} is not supported in 4 bits (64 and 128 are)")
+    _want(name, k_scales.dtype == v_scales.dtype == torch.bfloat16 and k_scales.shape == v_scales.shape == (pages, n_kv, page_size, 2),
+          "scales are bfloat16 [pages, key/value heads, page size, 2]")
+    _want(name, k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous(),
+          "the cache's tensors are contiguous")
+    return pages, n_kv, page_size, 2 * half
+
+
+def _indices(name: str, tensor: torch.Tensor, least: int, what: str) -> None:
+    _want(name, tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous() and tensor.shape[0] >= least, what)
+
+
+def rope_kv_write_int4(qkv: torch.Tensor, bias: torch.Tensor | None, positions: torch.Tensor, slot_mapping: torch.Tensor,
+                       inv_freq: torch.Tensor, q_out: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                       v_codes: torch.Tensor, v_scales: torch.Tensor, n_q: int, n_kv: int, head_dim: int, pairing: int) -> None:
+    """:func:`rope_kv_write` into a 4-bit cache: bias, rotary encoding of queries and keys, and the write of keys and values as
+    codes with a scale and a centre a row.  q_out bfloat16 [T, n_q, head_dim].  ``qkv`` is [T, width] in bfloat16 or float32, or a float32
+    stack of partial sums [P, T, width].  Angles, keys and values are worked out in 64 bits up to the code.  Rows with a slot of -1
+    are not cached; two rows of a step have different slots."""
+    name = "rope_kv_write_int4"
+    width = (n_q + 2 * n_kv) * head_dim
+    _want(name, qkv.dim() in (2, 3) and qkv.shape[-1] == width and qkv.stride(-1) == 1, f"projections have rows of {width} values")
+    tokens = qkv.shape[-2]
+    if qkv.dim() == 3:
+        _want(name, qkv.dtype == torch.float32 and qkv.is_contiguous(), "partial sums are contiguous float32")
+        n_partials, stride, row_stride = qkv.shape[0], tokens * width, width
+    else:
+        n_partials, stride, row_stride = 1, 0, qkv.stride(0) if tokens > 1 else width
+    code = dtype_code(qkv.dtype)
+    pages, heads, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
+    _want(name, heads == n_kv and dim == head_dim, f"the cache has {heads} heads of {dim}, the projections {n_kv} of {head_dim}")
+    _indices(name, positions, tokens, "positions are int32, one a row")
+    _indices(name, slot_mapping, tokens, "slots are int32, one a row")
+    _want(name, inv_freq.dtype == torch.float32 and inv_freq.shape == (head_dim // 2,) and inv_freq.is_contiguous(), "frequencies are float32 [head size / 2]")
+    _want(name, q_out.dtype == torch.bfloat16 and q_out.shape == (tokens, n_q, head_dim) and q_out.is_contiguous(),
+          "q_out is contiguous bfloat16 [rows, query heads, head size]")
+    _want(name, bias is None or (bias.dtype == torch.float32 and bias.shape == (width,) and bias.is_contiguous()), f"the bias is float32 [{width}]")
+    _here(name, qkv, bias, positions, slot_mapping, inv_freq, q_out, k_codes, k_scales, v_codes, v_scales)
+    check(library.load().lse_rope_kv_write_int4(qkv.data_ptr(), code, n_partials, stride, _ptr(bias), positions.data_ptr(),
+                                                slot_mapping.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(),
+                                                k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), tokens, n_q, n_kv,
+                                                head_dim, page_size, pairing, row_stride, pages, _stream()), name)
+
+
+def kv_read_int4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                 slot_mapping: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
+    """The keys and values that a 4-bit cache holds at the slots, as bfloat16 [T, n_kv, D]; rows with a slot of -1 are left alone."""
+    name = "kv_read_int4"
+    pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
+    tokens = k_out.shape[0]
+    for out in (k_out, v_out):
+        _want(name, out.dtype == torch.bfloat16 and out.shape == (tokens, n_kv, dim) and out.is_contiguous(),
+              f"outputs are contiguous bfloat16 [rows, {n_kv}, {dim}]")
+    _indices(name, slot_mapping, tokens, "slots are int32, one a row")
+    _here(name, k_codes, k_scales, v_codes, v_scales, slot_mapping, k_out, v_out)
+    check(library.load().lse_kv_read_int4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                                          slot_mapping.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), tokens, n_kv, dim, page_size,
+                                          pages, _stream()), name)
+
+
+def _int4_queries(name: str, q: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor, n_kv: int, dim: int, scale: float) -> None:
+    _want(name, q.dim() == 3 and q.dtype == out.dtype == torch.bfloat16 and out.shape == q.shape, "queries and outputs are bfloat16 [rows, heads, head size]")
+    _want(name, q.is_contiguous() and out.is_contiguous(), "queries and outputs are contiguous")
+    _want(name, q.shape[2] == dim and q.shape[1] % n_kv == 0, f"{q.shape[1]} query heads of {q.shape[2]} do not fit {n_kv} key/value heads of {dim}")
+    _want(name, block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block tables are int32 [requests, pages]")
+    _want(name, scale > 0.0, "the scale is positive")
+
+
+INT4_DECODE_BLOCKS = 4          # blocks that an SM holds
+INT4_DECODE_KEYS = 64           # keys of a part: a tile for each of a block's warps
+INT4_DECODE_CLUSTER = 8         # parts that one launch adds up; more take a second launch
+
+
+def decode_splits_int4(tokens: int, n_q: int, n_kv: int, max_context: int) -> int:
+    """How many parts the keys of a row are cut into: blocks for all SMs, a tile for each of their warps at least."""
+    base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
+    splits = max(1, min(sm_count() * INT4_DECODE_BLOCKS // base, -(-max_context // INT4_DECODE_KEYS)))
+    return splits
+
+
+def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                                v_scales: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor,
+                                segment_of_token: torch.Tensor, positions: torch.Tensor, scale: float, max_context: int = 0,
+                                num_splits: int | None = None) -> torch.Tensor:
+    """:func:`paged_attention_decode` over a 4-bit cache: every row of q (bfloat16 [T, n_q, D], D 64 or 128) attends to the keys
+    0 .. its position of its request.  Rows of segment -1 are left alone; a row at position -1 sees nothing and gets zeros.
+    ``max_context``: keys that any request holds at most (0: what the block tables have room for); it and the number of rows decide
+    into how many parts (``num_splits``) the keys are cut."""
+    name = "paged_attention_decode_int4"
+    pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
+    _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
+    tokens, n_q, _ = q.shape
+    _indices(name, segment_of_token, tokens, "segments are int32, one a row")
+    _indices(name, positions, tokens, "positions are int32, one a row")
+    _here(name, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_of_token, positions)
+    if tokens == 0:
+        return out
+    room = block_tables.shape[1] * page_size
+    if num_splits is None:
+        num_splits = decode_splits_int4(tokens, n_q, n_kv, min(room, max_context) if max_context > 0 else room)
+    scratch = None
+    if num_splits > INT4_DECODE_CLUSTER:
+        scratch = torch.empty(tokens * n_q * num_splits * (dim + 2), dtype=torch.float32, device=q.device)
+    check(library.load().lse_paged_attention_decode_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                                                         v_scales.data_ptr(), out.data_ptr(), _ptr(scratch), block_tables.data_ptr(),
+                                                         block_tables.stride(0), segment_of_token.data_ptr(), positions.data_ptr(),
+                                                         tokens, n_q, n_kv, dim, page_size, scale, num_splits, pages,
+                                                         block_tables.shape[0], _stream()), name)
+    return out
+
+
+# ------------------------------------------------------------------ beam search
+MAX_BEAMS = 32
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, ended: torch.Tensor, end_token: int, out_scores: torch.Tensor,
+                out_tokens: torch.Tensor, out_parents: torch.Tensor, out_ended: torch.Tensor) -> None:
+    """The K best continuations of each request's K beams, the best first (of equal ones the lower beam, then the lower token).
+
+    logits float32 [B * K, V] (rows may be strided); scores float32, ended int32 [B, K]: a beam's sum of log probabilities, and
+    whether it has ended.  A beam that goes on offers score + logit - logsumexp(logits) for every token, one that has ended
+    offers ``end_token`` at its own score, one of score -inf (or whose logits are not numbers) nothing.  Outputs [B, K]: scores
+    float32, tokens, parents (the beam within the request) and ended (int32: the parent had ended or the token is ``end_token``).
+    Where fewer than K are offered the rest are (-inf, end_token, their own number, 1)."""
+    name = "beam_select"
+    _want(name, scores.dim() == 2 and scores.dtype == torch.float32, "scores are float32 [requests, beams]")
+    requests, beams = scores.shape
+    _want(name, 1 <= beams <= MAX_BEAMS, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
+    _want(name, logits.dim() == 2 and logits.dtype == torch.float32 and logits.shape[0] == requests * beams and logits.shape[1] > 0
+          and logits.stride(1) == 1, "logits are float32 [requests * beams, vocabulary]")
+    vocab = logits.shape[1]
+    _want(name, 0 <= end_token < vocab, f"the end token {end_token} lies outside the vocabulary")
+    for tensor, kind in ((scores, torch.float32), (ended, torch.int32), (out_scores, torch.float32), (out_tokens, torch.int32),
+                         (out_parents, torch.int32), (out_ended, torch.int32)):
+        _want(name, tensor.dtype == kind and tensor.shape == (requests, beams) and tensor.is_contiguous(),
+              "scores are contiguous float32, the other arrays int32, all [requests, beams]")
+    _here(name, logits, scores, ended, out_scores, out_tokens, out_parents, out_ended)
+    if requests == 0:
+        return
+    lib = library.load()
+    scratch = torch.empty(1024 * lib.lse_beam_select_scratch_kb(requests, beams, vocab), dtype=torch.uint8, device=logits.device)
+    check(lib.lse_beam_select(logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, requests, beams, vocab,
+                              scores.data_ptr(), ended.data_ptr(), end_token, scratch.data_ptr(), out_scores.data_ptr(),
+                              out_tokens.data_ptr(), out_parents.data_ptr(), out_ended.data_ptr(), _stream()), name)
+
+
+MAX_REORDER_STORAGES = 24
+
+
+def beam_reorder(parents: torch.Tensor, block_tables: torch.Tensor, lengths: torch.Tensor, new_tables: torch.Tensor,
+                 page_size: int, storages: list) -> None:
+    """Block tables after :func:`beam_select`, and the copies of what two beams may no longer share.
+
+    parents int32 [B, K]; block_tables, new_tables int32 [B * K, W] (different tensors); lengths int32 [B]: tokens that the beams
+    of a request hold, all alike.  Beam i goes on from its parent's pages.  The page that is being filled (``length % page_size`` tokens
+    in it) goes to the parent's first child; further children take over that of a beam without a child, into which it is
+    copied.  Entries behind it are a row's own empty pages and stay.  ``storages``: tensors [outer, pages, ...], each page
+    contiguous (a group's storage as [layers * 2, pages, ...]; states as [1, slots, ...] with tables of one column, lengths of
+    1 and a page size of 2).  A page that is being filled belongs to one beam only."""
+    name = "beam_reorder"
+    _want(name, parents.dim() == 2 and parents.dtype == torch.int32 and parents.is_contiguous(), "parents are int32 [requests, beams]")
+    requests, beams = parents.shape
+    _want(name, 1 <= beams <= MAX_BEAMS, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
+    _want(name, page_size > 0, "the page size is positive")
+    for tables in (block_tables, new_tables):
+        _want(name, tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == requests * beams and tables.shape[1] > 0
+              and tables.stride(1) == 1 and tables.shape == block_tables.shape, "block tables are int32 [requests * beams, pages]")
+    _want(name, new_tables.data_ptr() != block_tables.data_ptr(), "the new tables are made in another tensor than the old ones")
+    _indices(name, lengths, requests, "lengths are int32, one a request")
+    numbers = []
+    for storage in storages:
+        _want(name, storage.dim() >= 3 and storage[0, 0].is_contiguous(), "storages are [outer, pages, ...] with contiguous pages")
+        size = storage.element_size()
+        numbers.append((storage.data_ptr(), storage.shape[0], storage.stride(0) * size, storage.stride(1) * size,
+                        storage[0, 0].numel() * size, storage.shape[1]))
+    _here(name, parents, block_tables, lengths, new_tables, *storages)
+    if requests == 0:
+        return
+    lib = library.load()
+    for at in range(0, max(1, len(numbers)), MAX_REORDER_STORAGES):
+        some = numbers[at:at + MAX_REORDER_STORAGES]
+        flat = (c_longlong * (6 * max(1, len(some))))(*(number for storage in some for number in storage))
+        check(lib.lse_beam_reorder(parents.data_ptr(), requests, beams, block_tables.data_ptr(), block_tables.stride(0),
+                                   block_tables.shape[1], lengths.data_ptr(), page_size, new_tables.data_ptr() if at == 0 else None,
+                                   new_tables.stride(0), flat, len(some), _stream()), name)
+
+
+def step_tables(first: torch.Tensor, counts: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, page_size: int,
+                segment_start: torch.Tensor, segment_of_token: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
+                contexts: torch.Tensor, block_tables: torch.Tensor) -> None:
+    """A step's arrays (``StepContext``) from its requests' lengths, made on the device.
+
+    Request s brings counts[s] tokens behind first[s] earlier ones and owns the pages pages[page_start[s] : page_start[s + 1]]
+    (all int32).  Written (int32): segment_start [S + 1], segment_of_token, positions and slot_mapping [T] (rows behind the last
+    request: -1, 0, -1; a row whose page is missing or -1: slot -1), contexts [S], block_tables [S, W] (-1 behind a request's pages)."""
+    name = "step_tables"
+    _indices(name, first, 1, "first positions are int32, one a request")
+    requests = first.shape[0]
+    _indices(name, counts, requests, "counts are int32, one a request")
+    _indices(name, page_start, requests + 1, "page starts are int32, one more than the requests")
+    _indices(name, pages, 0, "pages are int32")
+    _indices(name, segment_start, requests + 1, "segment starts are int32, one more than the requests")
+    _indices(name, contexts, requests, "contexts are int32, one a request")
+    tokens = segment_of_token.shape[0]
+    for rows in (segment_of_token, positions, slot_mapping):
+        _indices(name, rows, tokens, "segments, positions and slots are int32, one a row")
+    _want(name, page_size > 0, "the page size is positive")
+    _want(name, block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests
+          and block_tables.stride(1) == 1, "block tables are int32 [requests, pages]")
+    _here(name, first, counts, pages, page_start, segment_start, segment_of_token, positions, slot_mapping, contexts, block_tables)
+    width = block_tables.shape[1]
+    check(library.load().lse_step_tables(first.data_ptr(), counts.data_ptr(), pages.data_ptr(), page_start.data_ptr(), requests,
+                                         page_size, tokens, segment_start.data_ptr(), segment_of_token.data_ptr(),
+                                         positions.data_ptr(), slot_mapping.data_ptr(), contexts.data_ptr(), block_tables.data_ptr(),
+                                         max(width, block_tables.stride(0)), width, _stream()), name)
