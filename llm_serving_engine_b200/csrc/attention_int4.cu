@@ -79,7 +79,10 @@ attn_decode_int4_kernel(const __nv_bfloat16* __restrict__ q, const unsigned char
   const int gcount = min(HEADS, group - g0);
   const int split = blockIdx.z;
   const int seg = LSE_CHECKED(segment_of_token[t_row], -1, num_segments, -1, LSE_CHECK_SEGMENT);
-  if (seg < 0) return;             // a padding row (all blocks of its cluster leave together)
+  if (seg < 0) {                   // a padding row (all blocks of its cluster leave together)
+    pdl_wait();                    // (a launch without work must not end before the one before it)
+    return;
+  }
   const int ctx = positions[t_row] + 1;
   const int* bt = block_tables + (size_t)seg * bt_stride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -300,8 +303,8 @@ combine_parts_kernel(const float* __restrict__ part_o, const float2* __restrict_
   __shared__ float sum_o[8][D], sum_l[8], top[8];
   const int row = blockIdx.x, head = blockIdx.y, n_q = gridDim.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
-  if (segment_of_token[row] < 0) return;
   pdl_wait();
+  if (segment_of_token[row] < 0) return;
   const size_t base = ((size_t)row * n_q + head) * parts;
   float M = -INFINITY;
   for (int p = threadIdx.x; p < parts; p += 256) M = fmaxf(M, part_ml[base + p].x);

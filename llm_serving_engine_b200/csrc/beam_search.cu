@@ -11,6 +11,9 @@
 // merge: a block per request, from the chunks' leavings.  Offers are compared in 64 bits: two beams' offers can be closer than
 // float32 tells apart, and lse's error would decide.
 // What bounds the choice: the logits are read once, 4 bytes each.
+//
+// The last kernels of a step: the next step's read its metadata (token ids, block tables) before they wait for the kernels before
+// them.  So the kernels here that write metadata never let the next one start early.
 #include "common.cuh"
 
 namespace {
@@ -45,7 +48,7 @@ beam_chunk_kernel(const float* __restrict__ logits, long long row_stride, int vo
   __shared__ double part[CHUNK_THREADS / 32];
   __shared__ int count;
   __shared__ Best list[LIST];
-  pdl_launch_dependents();
+  pdl_launch_dependents();     // (merge: it waits before it reads anything)
   pdl_wait();
   const int row = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -161,7 +164,6 @@ beam_merge_kernel(const Best* __restrict__ best, const Sum* __restrict__ sums, i
   __shared__ long long list_at[LIST];
   __shared__ int over[MAX_BEAMS], count;
   __shared__ float score[MAX_BEAMS];
-  pdl_launch_dependents();
   pdl_wait();
   const int request = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)request * beams;
@@ -294,7 +296,6 @@ __global__ void __launch_bounds__(256)
 beam_reorder_kernel(const int* __restrict__ parents, int beams, const int* __restrict__ tables, int table_stride, int width,
                     const int* __restrict__ lengths, int page_size, int* __restrict__ new_tables, int new_stride,
                     const __grid_constant__ Storages storages) {
-  pdl_launch_dependents();
   pdl_wait();
   const int row = blockIdx.x, request = row / beams, beam = row - request * beams, lane = threadIdx.x & 31;
   // every warp works out all beams' sources, a beam a lane

@@ -5,6 +5,7 @@
 // Request s brings counts[s] tokens behind first[s] earlier ones and owns pages[page_start[s] .. page_start[s + 1]).  Every block
 // of the rows adds up all counts itself, 256 at a time (a step holds hundreds of requests at most), and looks its rows up in the
 // running sums, so one launch does it: what bounds it is the launch and two dependent loads, not the few hundred KB written.
+// The step's kernels read this metadata before they wait for the kernels before them, so this one never lets the next start early.
 #include "common.cuh"
 
 namespace {
@@ -17,7 +18,6 @@ step_tables_kernel(const int* __restrict__ first, const int* __restrict__ counts
                    int* __restrict__ segment_start, int* __restrict__ segment_of_token, int* __restrict__ positions,
                    int* __restrict__ slots, int* __restrict__ contexts, int* __restrict__ tables, int table_stride, int width) {
   __shared__ int ends[THREADS], warp_sums[THREADS / 32];
-  pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((int)blockIdx.x >= row_blocks) {       // block tables

@@ -672,12 +672,13 @@ def gemm_bf16_skinny_status() -> int:
 
 _STATUS_WORDS = (("gemm_tcgen05", "lse_gemm_bf16_skinny_status"), ("attention_tcgen05", "lse_attention_tc_status"),
                  ("attention_expanded_tcgen05", "lse_attention_expanded_status"), ("decode_layers", "lse_decode_layers_status"),
-                 ("gemm_pairs", "lse_gemm_pairs_status"))
+                 ("gemm_pairs", "lse_gemm_pairs_status"), ("attention_int4_tcgen05", "lse_attention_int4_tc_status"))
 
 
 def kernel_status_async(host_words: torch.Tensor) -> None:
     """Queue, on the current stream, copies of the status words of the kernels with bounded waits (the
-    few-rows product, the tcgen05 prompt attention, the one over expanded latents, the decode step in one launch, the product on pairs of SMs) into
+    few-rows product, the tcgen05 prompt attention, the one over expanded latents, the decode step in one launch, the product on pairs of SMs, the
+    prompt attention over 4-bit keys) into
     ``host_words`` (pinned int32, a word each; [2]: the first two).  Once the
     stream has got there, a non-zero word says that a wait gave up: that block wrote nothing, and
     what the step computed is not to be used."""
@@ -2220,6 +2221,54 @@ def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
                                                          block_tables.stride(0), segment_of_token.data_ptr(), positions.data_ptr(),
                                                          tokens, n_q, n_kv, dim, page_size, scale, num_splits, pages,
                                                          block_tables.shape[0], _stream()), name)
+    return out
+
+
+INT4_TILE = 128                              # keys of a tile, score rows of a block of the portions' kernel
+INT4_WORKSPACE_BYTES = 256 << 20             # most that keys and values expanded at a time take: beyond, some heads after the others
+
+
+def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                                 v_scales: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor, segment_start: torch.Tensor,
+                                 segment_first_position: torch.Tensor, scale: float, keys: int = 0, skip_single: bool = False,
+                                 max_portions: int = 0) -> torch.Tensor:
+    """:func:`paged_attention_prefill` over a 4-bit cache: prompt portions, causal, behind all earlier keys of their requests.
+
+    q, out bfloat16 [T, n_q, D], D 64 or 128, at most 128 query heads a key/value head; segment_start int32 [S + 1],
+    segment_first_position int32 [S].  ``keys``: keys that the requests hold together, at most (0: what the block tables have room
+    for); keys and values are worked on as float16 in a workspace of that size (a request beyond it comes out as NaN, as do rows
+    that attend to a value that float16 does not hold: 65,504; keys: 2^24).  ``skip_single``: requests of one row are left to
+    :func:`paged_attention_decode_int4`; ``max_portions`` (with it): at most so many requests have more."""
+    name = "paged_attention_prefill_int4"
+    pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
+    _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
+    tokens, n_q, _ = q.shape
+    segments = block_tables.shape[0]
+    group = n_q // n_kv
+    _want(name, group <= INT4_TILE, f"{group} query heads a key/value head: at most {INT4_TILE}")
+    _want(name, segments > 0, "block tables have a row a request")
+    _indices(name, segment_start, segments + 1, "segment starts are int32, one more than the requests")
+    _indices(name, segment_first_position, segments, "first positions are int32, one a request")
+    _here(name, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_start, segment_first_position)
+    if tokens == 0:
+        return out
+    room = segments * -(-block_tables.shape[1] * page_size // INT4_TILE)
+    capacity = min(room, keys // INT4_TILE + segments) if keys > 0 else room
+    a_head = capacity * INT4_TILE * dim
+    heads_at_once = min(n_kv, max(1, INT4_WORKSPACE_BYTES // (4 * a_head)))
+    with_tiles = min(segments, max_portions) if skip_single and max_portions > 0 else segments
+    # several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs
+    blocks = (-(-tokens // (INT4_TILE // group)) + with_tiles) * heads_at_once
+    parts = max(1, min(8, 5 * sm_count() // (4 * blocks)))
+    workspace = torch.empty(2 * heads_at_once * a_head, dtype=torch.float16, device=q.device)
+    scratch = torch.empty(tokens * n_q * parts * (dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+    at = workspace.data_ptr()
+    check(library.load().lse_paged_attention_prefill_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                                                          v_scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(),
+                                                          block_tables.stride(0), segment_start.data_ptr(),
+                                                          segment_first_position.data_ptr(), segments, tokens, pages, n_q, n_kv, dim,
+                                                          page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts,
+                                                          at, at + 2 * heads_at_once * a_head, _ptr(scratch), _stream()), name)
     return out
 
 

@@ -262,3 +262,130 @@ def test_rows_captured_and_on_another_stream():
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
         positions.copy_(torch.tensor([600, 77]).int())
+
+
+# ------------------------------------------------------------------ attention of prompt portions
+def f16_bound(expected, weighed):
+    """The result's rounding (2^-8 of it); values and weights in float16 (2^-11 of every term each); keys in float16, which move a score
+    by up to 2^-11 of the sum of |q k| (see ``portions``: given there as a factor of the terms)."""
+    return 2.0 ** -8 * expected.abs() + (2.0 ** -10 + 2.0 ** -14) * weighed + 1e-30
+
+
+def portions(cache, tables, counts, firsts, q, out, scale, page_size, skip_single=False):
+    """Every row of ``out`` against the plain form; returns how many were compared."""
+    row, compared = 0, 0
+    for s, (count, first) in enumerate(zip(counts, firsts)):
+        if count:
+            k, v = request_rows(cache, tables[s], first + count, page_size)
+        for i in range(count):
+            if not (skip_single and count == 1) and (i < 3 or i >= count - 3 or i % 29 == 0):
+                expected, weighed = plain.attend(q[row], k, v, first + i, scale)
+                # a key's rounding moves a score by at most 2^-11 sum |q k| scale, up and down: twice that in a weight's share
+                reach = torch.einsum("hd,nhd->hn", q[row].to(D64).abs(), k[:first + i + 1].abs().repeat_interleave(q.shape[1] // k.shape[1], 1)).amax(-1) * scale
+                assert ((out[row].to(D64) - expected).abs() <= f16_bound(expected, weighed) + 2.0 ** -10 * reach[:, None] * weighed).all(), (s, i)
+                compared += 1
+            row += 1
+    return compared
+
+
+def portion_case(counts, firsts, n_kv, dim, page_size, seed):
+    g = torch.Generator().manual_seed(seed)
+    held = [-(-(n + f) // page_size) if n else 0 for n, f in zip(counts, firsts)]
+    cache = fill_cache(g, sum(held) + 1, n_kv, page_size, dim)
+    order = torch.randperm(sum(held), generator=g).tolist()
+    tables = torch.full((len(counts), max(held) + 1), -1, dtype=torch.int32)
+    for s, n in enumerate(held):
+        tables[s, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=torch.int32)
+        if n:      # what lies behind the last key is anything at all
+            rest = counts[s] + firsts[s] - (n - 1) * page_size
+            for scales in (cache[1], cache[3]):
+                scales[int(tables[s, n - 1]), :, rest:] = math.nan
+    start = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()]).int().cuda()
+    return g, cache, tables.cuda(), start, torch.tensor(firsts).int().cuda()
+
+
+@pytest.mark.parametrize("counts,firsts,n_q,n_kv,dim,page_size", [
+    ([1], [0], 2, 2, 64, 16), ([130], [0], 4, 4, 128, 16), ([3, 1, 0, 40], [5, 0, 0, 700], 12, 2, 128, 16), ([200, 77, 2], [0, 300, 1500], 28, 4, 128, 8),
+    ([5], [4000], 40, 8, 128, 32), ([260], [33], 7, 1, 64, 5), ([129, 128, 127], [127, 128, 1], 5, 5, 64, 128), ([20, 9], [0, 250], 128, 1, 64, 16),
+    ([400], [2000], 9, 3, 128, 24)])
+def test_portions(counts, firsts, n_q, n_kv, dim, page_size):
+    g, cache, tables, start, first = portion_case(counts, firsts, n_kv, dim, page_size, sum(counts))
+    tokens = sum(counts)
+    q = (1.5 * torch.randn((tokens + 3, n_q, dim), generator=g)).bfloat16().cuda()
+    scale = dim ** -0.5
+    for keys in (0, sum(counts) + sum(firsts)):
+        out = torch.full_like(q, 3.0)
+        ops.paged_attention_prefill_int4(q, *cache, out, tables, start, first, scale, keys=keys)
+        assert portions(cache, tables, counts, firsts, q, out, scale, page_size) >= min(tokens, 5)
+        assert (out[tokens:] == 3.0).all()          # rows behind the last sequence
+    single = torch.full_like(q, 3.0)
+    ops.paged_attention_prefill_int4(q, *cache, single, tables, start, first, scale, skip_single=True, max_portions=sum(n > 1 for n in counts))
+    row = 0
+    for n in counts:
+        assert (single[row:row + n] == 3.0).all() if n == 1 else torch.equal(single[row:row + n], out[row:row + n])
+        row += n
+
+
+def test_portions_some_heads_at_a_time(monkeypatch):
+    counts, firsts = [50, 30], [300, 0]
+    g, cache, tables, start, first = portion_case(counts, firsts, 5, 64, 16, 1)
+    q = torch.randn((80, 10, 64), generator=g).bfloat16().cuda()
+    want = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.125)
+    monkeypatch.setattr(ops, "INT4_WORKSPACE_BYTES", 1)
+    out = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.125)
+    portions(cache, tables, counts, firsts, q, out, 0.125, 16)
+    portions(cache, tables, counts, firsts, q, want, 0.125, 16)
+
+
+def test_portions_with_scores_far_apart():
+    """Maxima that grow by more than float16 reaches from one tile to the next."""
+    counts, firsts = [300], [600]
+    g, cache, tables, start, first = portion_case(counts, firsts, 1, 128, 16, 2)
+    pages = tables[0, :57].long()
+    ramp = torch.linspace(0.05, 6.0, 57).view(-1, 1, 1).cuda()
+    cache[1][pages, :, :, 0] = (ramp * cache[1][pages, :, :, 0].float().nan_to_num(0.3)).bfloat16()
+    cache[1][pages, :, :, 1] = 0.0
+    q = (4 * torch.randn((300, 6, 128), generator=g)).bfloat16().cuda()
+    out = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.09)
+    portions(cache, tables, counts, firsts, q, out, 0.09, 16)
+
+
+def test_portions_reach_of_what_is_not_a_number():
+    """A key or value that is not a number, or beyond float16, reaches the rows that see it and no others."""
+    for index, wrong in ((1, math.nan), (3, math.nan), (3, 1e5), (3, math.inf), (1, 1e8)):
+        counts, firsts = [140], [20]
+        g, cache, tables, start, first = portion_case(counts, firsts, 2, 64, 16, 3)
+        cache[index][int(tables[0, 5]), 1, 4, 1] = wrong          # position 84 of head 1
+        q = torch.randn((140, 4, 64), generator=g).bfloat16().cuda()
+        out = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.125)
+        sees = torch.arange(20, 160).cuda() >= 84
+        assert torch.isfinite(out[:, :2].float()).all() and torch.isfinite(out[~sees].float()).all() and out[sees][:, 2:].isnan().all()
+
+
+def test_portions_beyond_the_announced_keys_are_not_made_up():
+    counts, firsts = [10, 10, 10], [300, 300, 300]
+    g, cache, tables, start, first = portion_case(counts, firsts, 1, 64, 16, 4)
+    q = torch.randn((30, 2, 64), generator=g).bfloat16().cuda()
+    out = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.125, keys=310)     # room for 2 + 3 tiles, 9 are held
+    assert torch.isfinite(out[:10].float()).all() and out[10:].isnan().all()
+
+
+def test_portions_captured():
+    counts, firsts = [33, 64], [500, 10]
+    g, cache, tables, start, first = portion_case(counts, firsts, 2, 128, 16, 5)
+    q = torch.randn((97, 8, 128), generator=g).bfloat16().cuda()
+    outs, graphs = [torch.empty_like(q) for _ in range(2)], []
+    want = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.09)
+    for out in outs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention_prefill_int4(q, *cache, out, tables, start, first, 0.09)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for graph, stream in zip(graphs, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
