@@ -75,7 +75,9 @@ __device__ __forceinline__ int tiles_before(const int* __restrict__ segment_star
 }
 
 // ------------------------------------------------------------------ expand
-// One block = 128 keys (a tile) of one head, keys or values; 256 threads, LANES = D / 8 of them a row, eight values each.
+// One block = EXPAND_KEYS keys of a tile and one head, keys and values; 256 threads, LANES = D / 8 of them a row, eight values each, all loads
+// of a thread on their way together (a block a tile, eight rows a thread one after the other: 17 us for 51 tiles of two heads).
+constexpr int EXPAND_KEYS = 32;
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat162* __restrict__ k_scales,
@@ -83,7 +85,7 @@ expand_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat1
                    uint4* __restrict__ v_out, const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
                    const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size, int num_pages, int capacity,
                    int skip_single) {
-  constexpr int LANES = D / 8, ROWS = 256 / LANES;
+  constexpr int LANES = D / 8, ROWS = 256 / LANES, MINE = EXPAND_KEYS / ROWS;      // rows at once, rows of a thread
   __shared__ int found[3];
   pdl_launch_dependents();
   const int tile = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -119,35 +121,45 @@ expand_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat1
   const int seg = found[0], key0 = found[1], keys = found[2];
   pdl_wait();                // (before any return: a launch without work must not end before the one before it)
   if (seg < 0) return;       // behind the last request's tiles, or one that another kernel takes
-  const int c = tid % LANES;
+  const int c = tid % LANES, r0 = blockIdx.z * EXPAND_KEYS + tid / LANES;
   const size_t out0 = ((size_t)head * capacity + tile) * BN;
   const int* bt = block_tables + (size_t)seg * bt_stride;
-#pragma unroll 4
-  for (int r = tid / LANES; r < BN; r += ROWS) {
-    const int key = key0 + r;
-    uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
-    if (key < keys) {
-      const int page = LSE_CHECKED(bt[key / page_size], 0, num_pages, 0, LSE_CHECK_TABLE_ENTRY);
-      const size_t place = ((size_t)page * n_kv + head0 + head) * page_size + key % page_size;
-      const uint32_t kx = __ldcs(reinterpret_cast<const uint32_t*>(k_codes + place * (D / 2)) + c);
-      const uint32_t vx = __ldcs(reinterpret_cast<const uint32_t*>(v_codes + place * (D / 2)) + c);
-      float2 ks = __bfloat1622float2(k_scales[place]);
-      const float2 vs = __bfloat1622float2(v_scales[place]);
-      ks.x *= KEY_SCALE; ks.y *= KEY_SCALE;
-      // the largest magnitude that the row's codes could stand for; false for what is not a number
-      const bool fits = fabsf(ks.y) + 8.f * fabsf(ks.x) <= 65504.f && fabsf(vs.y) + 8.f * fabsf(vs.x) <= 65504.f;
-      auto values = [](uint32_t x, float2 s) {
-        uint32_t w[4];
+  uint32_t kx[MINE], vx[MINE];
+  __nv_bfloat162 ks[MINE], vs[MINE];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = pack_f16(fmaf(s.x, (float)((int)(x >> (8 * j) & 15u) - 8), s.y), fmaf(s.x, (float)((int)(x >> (8 * j + 4) & 15u) - 8), s.y));
-        return make_uint4(w[0], w[1], w[2], w[3]);
-      };
-      if (fits) { kw = values(kx, ks); vw = values(vx, vs); }
-      else kw = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);
+  for (int i = 0; i < MINE; ++i) {
+    const int key = key0 + r0 + i * ROWS;
+    kx[i] = vx[i] = 0u;
+    ks[i] = vs[i] = __floats2bfloat162_rn(0.f, 0.f);      // (keys behind the last become zeros)
+    if (key < keys) {
+      const int logical = (unsigned)key / (unsigned)page_size;
+      const int page = LSE_CHECKED(bt[logical], 0, num_pages, 0, LSE_CHECK_TABLE_ENTRY);
+      const size_t place = ((size_t)page * n_kv + head0 + head) * page_size + (key - logical * page_size);
+      kx[i] = __ldcs(reinterpret_cast<const uint32_t*>(k_codes + place * (D / 2)) + c);
+      vx[i] = __ldcs(reinterpret_cast<const uint32_t*>(v_codes + place * (D / 2)) + c);
+      ks[i] = k_scales[place];
+      vs[i] = v_scales[place];
     }
-    k_out[(out0 + r) * LANES + c] = kw;
-    v_out[(out0 + r) * LANES + c] = vw;
+  }
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    float2 kf = __bfloat1622float2(ks[i]);
+    const float2 vf = __bfloat1622float2(vs[i]);
+    kf.x *= KEY_SCALE; kf.y *= KEY_SCALE;
+    // the largest magnitude that the row's codes could stand for; false for what is not a number
+    const bool fits = fabsf(kf.y) + 8.f * fabsf(kf.x) <= 65504.f && fabsf(vf.y) + 8.f * fabsf(vf.x) <= 65504.f;
+    auto values = [](uint32_t x, float2 s) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = pack_f16(fmaf(s.x, (float)((int)(x >> (8 * j) & 15u) - 8), s.y), fmaf(s.x, (float)((int)(x >> (8 * j + 4) & 15u) - 8), s.y));
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    uint4 kw = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u), vw = make_uint4(0, 0, 0, 0);
+    if (fits) { kw = values(kx[i], kf); vw = values(vx[i], vf); }
+    const size_t at = (out0 + r0 + i * ROWS) * LANES + c;
+    k_out[at] = kw;
+    v_out[at] = vw;
   }
 }
 
@@ -556,7 +568,7 @@ int launch_portions(const void* q, const void* k_codes, const void* k_scales, co
         !make_map_row_groups(&map_k, keys, (long long)heads * capacity * BN, D, BN) ||
         !make_map_row_groups(&map_v, values, (long long)heads * capacity * BN, D, BN))
       return LSE_ERR_BAD_ARGUMENT;
-    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads), dim3(256), 0, stream, (const unsigned char*)k_codes,
+    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads, BN / EXPAND_KEYS), dim3(256), 0, stream, (const unsigned char*)k_codes,
                      (const __nv_bfloat162*)k_scales, (const unsigned char*)v_codes, (const __nv_bfloat162*)v_scales, (uint4*)keys,
                      (uint4*)values, block_tables, bt_stride, segment_start, first_pos, num_segments, n_kv, head0, page_size,
                      (int)num_pages, capacity, skip_single);

@@ -36,128 +36,181 @@ __device__ __forceinline__ double shfl_xor_double(double v, int o) {
 // double to bfloat16 by way of float32, as a tensor library converts
 __device__ __forceinline__ __nv_bfloat16 bf16_of(double v) { return __float2bfloat16_rn((float)v); }
 
-// One block = one token x a range of heads (queries, then keys, then values).  A thread owns eight values of a head: pairing 0
-// the neighbours 8 c .. 8 c + 7 (four pairs), pairing 1 the runs 4 c .. and D / 2 + 4 c .. (pairs across the halves).
-// LANES = D / 8 threads share a head and find its extremes by shuffles.
-template <typename TI, int D, int PAIRING>
-__global__ void __launch_bounds__(256)
+// One block = TOKENS tokens x their query heads (blockIdx.y < q_blocks), or x their key and value heads.  It works out the tokens' sines
+// (a thread each), then its threads walk (token, head) rows with the next row's projections on their way.  A thread owns eight
+// values of a head: pairing 0 the neighbours 8 c .. 8 c + 7 (four pairs), pairing 1 the runs 4 c .. and D / 2 + 4 c .. (pairs across
+// the halves).  LANES = D / 8 threads share a head and find its extremes by shuffles.
+// What bounds it: the instructions of the 64-bit part.  2,001 rows of 40 / 8 heads of 128 in float32 (90 MB) take 27 us, 41 with a block
+// that walked all heads of a token in 64 bits, one pass after the other.
+constexpr int THREADS = 256;
+template <typename TI, int D, int PAIRING, int TOKENS>
+__global__ void __launch_bounds__(THREADS, 4)
 rope_kv_write_int4_kernel(const TI* __restrict__ qkv, int n_partials, long long partial_stride, const float* __restrict__ bias,
                           const int* __restrict__ positions, const int* __restrict__ slot_mapping,
                           const float* __restrict__ inv_freq, __nv_bfloat16* __restrict__ q_out, unsigned char* __restrict__ k_codes,
                           __nv_bfloat162* __restrict__ k_scales, unsigned char* __restrict__ v_codes,
-                          __nv_bfloat162* __restrict__ v_scales, int n_q, int n_kv, int page_size, long long qkv_stride,
-                          long long num_slots, int heads_a_block) {
-  constexpr int LANES = D / 8, HALF = D / 2;
-  __shared__ double2 turn_s[HALF];      // cosine and sine of the token's angles
+                          __nv_bfloat162* __restrict__ v_scales, int tokens, int n_q, int n_kv, int page_size, long long qkv_stride,
+                          long long num_slots, int q_blocks) {
+  constexpr int LANES = D / 8, HALF = D / 2, HEADS = THREADS / LANES;
+  __shared__ double2 turn_s[TOKENS * HALF];      // cosines and sines of the tokens' angles
   pdl_launch_dependents();
-  const int t = blockIdx.x;
-  const int heads = n_q + 2 * n_kv;
-  const int first_head = blockIdx.y * heads_a_block, last_head = min(heads, first_head + heads_a_block);
-  // position, slot and frequencies are the step's own data: read before the wait for the kernel that makes the projections
-  const int slot = LSE_CHECKED(slot_mapping[t], -1, (int)num_slots, -1, LSE_CHECK_CACHE_SLOT);
-  if (first_head < n_q + n_kv)
-    for (int i = threadIdx.x; i < HALF; i += blockDim.x) {
-      double angle = (double)positions[t] * (double)inv_freq[i];
-      angle -= 6.283185307179586 * rint(angle * 0.15915494309189535);
+  const int t0 = blockIdx.x * TOKENS, count = min(TOKENS, tokens - t0);
+  const bool queries = (int)blockIdx.y < q_blocks;
+  const int heads = queries ? n_q : 2 * n_kv, head0 = queries ? 0 : n_q;         // of a token; its first among a row's heads
+  const int step = HEADS * (queries ? q_blocks : (int)gridDim.y - q_blocks), rows = count * heads;
+  const int begin = (queries ? (int)blockIdx.y : (int)blockIdx.y - q_blocks) * HEADS;
+  const int c = threadIdx.x % LANES;
+  const int e0 = PAIRING == 0 ? 8 * c : 4 * c, e1 = PAIRING == 0 ? 8 * c + 4 : HALF + 4 * c;
+  // positions, slots, frequencies and bias are the step's or the model's own data: read before the wait for the kernel that makes the
+  // projections
+  for (int i = threadIdx.x; i < count * HALF; i += THREADS) {
+    double angle = (double)positions[t0 + i / HALF] * (double)inv_freq[i % HALF];
+    angle -= 6.283185307179586 * rint(angle * 0.15915494309189535);
+    if (queries) {
+      float sn, cs;
+      sincosf((float)angle, &sn, &cs);
+      reinterpret_cast<float2*>(turn_s)[i] = make_float2(cs, sn);
+    } else {
       double sn, cs;
       sincos(angle, &sn, &cs);
       turn_s[i] = make_double2(cs, sn);
     }
-  __syncthreads();
+  }
   pdl_wait();
-  const int c = threadIdx.x % LANES, rows_at_once = blockDim.x / LANES;
-  const int e0 = PAIRING == 0 ? 8 * c : 4 * c, e1 = PAIRING == 0 ? 8 * c + 4 : HALF + 4 * c;
-  // all lanes of a warp stay in the loop: the shuffles take whole warps
-  for (int base = first_head; base < last_head; base += rows_at_once) {
-    const int head = base + threadIdx.x / LANES;
-    const bool is_q = head < n_q, is_k = !is_q && head < n_q + n_kv;
-    const bool live = head < last_head && (is_q || slot >= 0);
-    float g0[4] = {0.f, 0.f, 0.f, 0.f}, g1[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const TI* row = qkv + (size_t)t * qkv_stride + (size_t)head * D;
-      for (int p = 0; p < n_partials; ++p) {
-        float a[4], b[4];
-        load_four<TI>(row + (size_t)p * partial_stride + e0, a);
-        load_four<TI>(row + (size_t)p * partial_stride + e1, b);
+  auto load_eight = [&](const auto* p, float (&to)[8]) {
+    float lo[4], hi[4];
+    load_four(p + e0, lo);
+    load_four(p + e1, hi);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { g0[j] += a[j]; g1[j] += b[j]; }
+    for (int j = 0; j < 4; ++j) { to[j] = lo[j]; to[4 + j] = hi[j]; }
+  };
+  struct Place { int row, token, head; };      // of this thread's row; head counted from head0
+  auto load_row = [&](const Place& p, float (&to)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to[j] = 0.f;
+    if (p.row >= rows) return;
+    const TI* row = qkv + (size_t)(t0 + p.token) * qkv_stride + (size_t)(head0 + p.head) * D;
+    if (n_partials == 1) {
+      load_eight(row, to);
+      return;
+    }
+#pragma unroll 4
+    for (int k = 0; k < n_partials; ++k) {
+      float a[8];
+      load_eight(row + (size_t)k * partial_stride, a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] += a[j];
+    }
+  };
+  auto at_row = [&](int row) { Place p; p.row = row; p.token = (unsigned)row / (unsigned)heads; p.head = row - p.token * heads; return p; };
+  Place now = at_row(begin + threadIdx.x / LANES);
+  float g[8];
+  load_row(now, g);
+  __syncthreads();
+  for (int base = begin; base < rows; base += step) {      // the same in the whole block: shuffles take whole warps
+    const Place next = at_row(now.row + step);
+    float ahead[8];
+    load_row(next, ahead);
+    float b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+    if (now.row < rows && bias) load_eight(bias + (size_t)(head0 + now.head) * D, b);
+    if (queries) {
+      if (now.row < rows) {
+        const float2* turn = reinterpret_cast<const float2*>(turn_s) + now.token * HALF + 4 * c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += b[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float& x = PAIRING == 0 ? g[2 * j] : g[j];
+          float& y = PAIRING == 0 ? g[2 * j + 1] : g[4 + j];
+          const float rx = x * turn[j].x - y * turn[j].y, ry = y * turn[j].x + x * turn[j].y;
+          x = rx; y = ry;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(g[2 * j], g[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        __nv_bfloat16* dst = q_out + ((size_t)t0 * n_q + now.row) * D;
+        if (PAIRING == 0) {
+          *reinterpret_cast<uint4*>(dst + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
+        }
       }
-    }
-    float b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live && bias) {
-      load_four<float>(bias + (size_t)head * D + e0, b0);
-      load_four<float>(bias + (size_t)head * D + e1, b1);
-    }
-    if (is_q && live) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { x[j] = g0[j] + b0[j]; x[4 + j] = g1[j] + b1[j]; }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double2 turn = turn_s[4 * c + j];
-        const float cs = (float)turn.x, sn = (float)turn.y;
-        float& a = PAIRING == 0 ? x[2 * j] : x[j];
-        float& b = PAIRING == 0 ? x[2 * j + 1] : x[4 + j];
-        const float ra = a * cs - b * sn, rb = b * cs + a * sn;
-        a = ra; b = rb;
-      }
-      __nv_bfloat16* dst = q_out + ((size_t)t * n_q + head) * D;
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-      *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
-    }
-    if (base + rows_at_once <= n_q) continue;     // the same for the whole block: queries only
-    double x[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { x[j] = (double)g0[j] + (double)b0[j]; x[4 + j] = (double)g1[j] + (double)b1[j]; }
-    if (is_k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double2 turn = turn_s[4 * c + j];
-        double& a = PAIRING == 0 ? x[2 * j] : x[j];
-        double& b = PAIRING == 0 ? x[2 * j + 1] : x[4 + j];
-        const double ra = a * turn.x - b * turn.y, rb = b * turn.x + a * turn.y;
-        a = ra; b = rb;
-      }
-    }
-    double low = x[0], high = x[0];
-    bool finite = isfinite(x[0]);
-#pragma unroll
-    for (int j = 1; j < 8; ++j) { low = fmin(low, x[j]); high = fmax(high, x[j]); finite = finite && isfinite(x[j]); }
-    int whole = finite ? 1 : 0;
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) {
-      low = fmin(low, shfl_xor_double(low, o));
-      high = fmax(high, shfl_xor_double(high, o));
-      whole &= __shfl_xor_sync(0xffffffffu, whole, o);
-    }
-    if (is_q || !live) continue;
-    __nv_bfloat16 scale = bf16_of((high - low) / 15.0);
-    __nv_bfloat16 centre = bf16_of(low + 8.0 * (double)__bfloat162float(scale));
-    if (!whole) { scale = __float2bfloat16_rn(0.f); centre = __float2bfloat16_rn(__int_as_float(0x7fc00000)); }
-    const double s = (double)__bfloat162float(scale), m = (double)__bfloat162float(centre);
-    uint32_t code[2] = {0u, 0u};      // four codes each: those of e0 .., those of e1 ..
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double step = whole && s != 0.0 ? rint((x[j] - m) / s) : 0.0;
-      const int u = (int)fmin(fmax(step + 8.0, 0.0), 15.0);
-      code[j >> 2] |= (uint32_t)u << (4 * (j & 3));
-    }
-    const size_t page = slot / page_size, off = slot % page_size;
-    const size_t place = (page * n_kv + (is_k ? head - n_q : head - n_q - n_kv)) * page_size + off;
-    unsigned char* dst = (is_k ? k_codes : v_codes) + place * (D / 2);
-    if (PAIRING == 0) {
-      *reinterpret_cast<uint32_t*>(dst + 4 * c) = code[0] | code[1] << 16;
     } else {
-      *reinterpret_cast<unsigned short*>(dst + 2 * c) = (unsigned short)code[0];
-      *reinterpret_cast<unsigned short*>(dst + D / 4 + 2 * c) = (unsigned short)code[1];
+      const bool is_k = now.head < n_kv;
+      const int slot = now.row < rows ? LSE_CHECKED(slot_mapping[t0 + now.token], -1, (int)num_slots, -1, LSE_CHECK_CACHE_SLOT) : -1;
+      double x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (double)g[j];
+      if (bias) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += (double)b[j];
+      }
+      if (is_k && now.row < rows) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double2 turn = turn_s[now.token * HALF + 4 * c + j];
+          double& p = PAIRING == 0 ? x[2 * j] : x[j];
+          double& q = PAIRING == 0 ? x[2 * j + 1] : x[4 + j];
+          const double rp = p * turn.x - q * turn.y, rq = q * turn.x + p * turn.y;
+          p = rp; q = rq;
+        }
+      }
+      double low = x[0], high = x[0], all = x[0] * 0.0;      // `all`: zero where every value is finite
+#pragma unroll
+      for (int j = 1; j < 8; ++j) {
+        low = x[j] < low ? x[j] : low;
+        high = x[j] > high ? x[j] : high;
+        all = fma(x[j], 0.0, all);
+      }
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) {
+        const double l = shfl_xor_double(low, o), h = shfl_xor_double(high, o);
+        low = l < low ? l : low;
+        high = h > high ? h : high;
+      }
+      // a row's lanes are LANES neighbours of a warp
+      const unsigned mine = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+      const bool whole = (__ballot_sync(0xffffffffu, all == 0.0) & mine) == mine;
+      if (slot >= 0) {
+        __nv_bfloat16 scale = bf16_of((high - low) / 15.0);
+        __nv_bfloat16 centre = bf16_of(low + 8.0 * (double)__bfloat162float(scale));
+        if (!whole) { scale = __float2bfloat16_rn(0.f); centre = __float2bfloat16_rn(__int_as_float(0x7fc00000)); }
+        const double s = (double)__bfloat162float(scale), m = (double)__bfloat162float(centre);
+        const double inverse = s != 0.0 ? 1.0 / s : 0.0;
+        uint32_t code[2] = {0u, 0u};      // four codes each: those of e0 .., those of e1 ..
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          // the quotient (x - c) / s to nearest, halves to even: its estimate is off by one at most, and what is left of x decides
+          // (exactly: rows that come in bfloat16 do lie half way between two codes)
+          const double from_centre = x[j] - m;
+          int q = whole ? __double2int_rn(from_centre * inverse) : 0;
+          const double twice = 2.0 * fma(-(double)q, s, from_centre);
+          if (twice > s || (twice == s && (q & 1))) ++q;
+          else if (twice < -s || (twice == -s && (q & 1))) --q;
+          if (!whole || s == 0.0) q = 0;
+          code[j >> 2] |= (uint32_t)(min(max(q, -8), 7) + 8) << (4 * (j & 3));
+        }
+        const size_t page = (unsigned)slot / (unsigned)page_size, off = (unsigned)slot % (unsigned)page_size;
+        const size_t place = (page * n_kv + (is_k ? now.head : now.head - n_kv)) * page_size + off;
+        unsigned char* dst = (is_k ? k_codes : v_codes) + place * (D / 2);
+        if (PAIRING == 0) {
+          *reinterpret_cast<uint32_t*>(dst + 4 * c) = code[0] | code[1] << 16;
+        } else {
+          *reinterpret_cast<unsigned short*>(dst + 2 * c) = (unsigned short)code[0];
+          *reinterpret_cast<unsigned short*>(dst + D / 4 + 2 * c) = (unsigned short)code[1];
+        }
+        if (c == 0) (is_k ? k_scales : v_scales)[place] = __nv_bfloat162(scale, centre);
+      }
     }
-    if (c == 0) (is_k ? k_scales : v_scales)[place] = __nv_bfloat162(scale, centre);
+    now = next;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = ahead[j];
   }
 }
 
@@ -195,16 +248,17 @@ int launch_write(const void* qkv, int n_partials, long long partial_stride, cons
                  const int* slot_mapping, const float* inv_freq, void* q_out, void* k_codes, void* k_scales, void* v_codes,
                  void* v_scales, int tokens, int n_q, int n_kv, int page_size, int pairing, long long qkv_stride,
                  long long num_slots, cudaStream_t stream) {
-  const int heads = n_q + 2 * n_kv, rows_at_once = 256 / (D / 8);
-  // few tokens: a block for every pass over the heads, so that the launch is one round trip long; many: a token's sines once
-  const int heads_a_block = tokens <= 512 ? rows_at_once : heads;
-  const dim3 grid((unsigned)tokens, (unsigned)((heads + heads_a_block - 1) / heads_a_block));
-#define LSE_INT4_WRITE(PAIRING)                                                                                          \
-  lse_launch(rope_kv_write_int4_kernel<TI, D, PAIRING>, grid, dim3(256), 0, stream, (const TI*)qkv, n_partials, partial_stride, \
+  constexpr int HEADS = THREADS / (D / 8);
+  // many tokens: four a block, whose angles take all its threads; few: a block for every pass over a token's heads
+  const bool many = tokens >= 512;
+  const int q_blocks = many ? 1 : (n_q + HEADS - 1) / HEADS, kv_blocks = many ? 1 : (2 * n_kv + HEADS - 1) / HEADS;
+  const dim3 grid((unsigned)(many ? (tokens + 3) / 4 : tokens), (unsigned)(q_blocks + kv_blocks));
+#define LSE_INT4_WRITE(PAIRING, TOKENS)                                                                                  \
+  lse_launch(rope_kv_write_int4_kernel<TI, D, PAIRING, TOKENS>, grid, dim3(THREADS), 0, stream, (const TI*)qkv, n_partials, partial_stride, \
              bias, positions, slot_mapping, inv_freq, (__nv_bfloat16*)q_out, (unsigned char*)k_codes,                   \
-             (__nv_bfloat162*)k_scales, (unsigned char*)v_codes, (__nv_bfloat162*)v_scales, n_q, n_kv, page_size, qkv_stride, \
-             num_slots, heads_a_block)
-  const cudaError_t err = pairing == 0 ? LSE_INT4_WRITE(0) : LSE_INT4_WRITE(1);
+             (__nv_bfloat162*)k_scales, (unsigned char*)v_codes, (__nv_bfloat162*)v_scales, tokens, n_q, n_kv, page_size, qkv_stride, \
+             num_slots, q_blocks)
+  const cudaError_t err = pairing == 0 ? (many ? LSE_INT4_WRITE(0, 4) : LSE_INT4_WRITE(0, 1)) : (many ? LSE_INT4_WRITE(1, 4) : LSE_INT4_WRITE(1, 1));
 #undef LSE_INT4_WRITE
   if (err != cudaSuccess) return (int)err;
   LSE_LAUNCH_CHECK();

@@ -2094,35 +2094,42 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
 # ------------------------------------------------------------------ keys and values in 4 bits
 # A row of D values of a head is held as codes u in 0 .. 15 (uint8 [pages, n_kv, page_size, D / 2], byte b: d = 2 b low, 2 b + 1 high)
 # with a scale s and a centre c (bfloat16 [pages, n_kv, page_size, 2]) and stands for s (u - 8) + c.
-def _want(name: str, ok: bool, what: str) -> None:
-    if not ok:
-        raise KernelError(f"{name}: {what}")
+def _refuse(name: str, what: str) -> None:
+    raise KernelError(f"{name}: {what}")
 
 
-def _here(name: str, *tensors: torch.Tensor) -> None:
-    """CUDA tensors of the current device: a kernel is launched on that one's stream."""
+_I32, _U8, _BF16, _FLOAT = torch.int32, torch.uint8, torch.bfloat16, torch.float32
+_get_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _elsewhere(name: str, device: int, *tensors: torch.Tensor) -> None:
+    """Raises for the tensor that does not lie on the current device, on whose stream a kernel is launched."""
     _need_cuda(*tensors)
-    device = torch._C._cuda_getDevice()
     for tensor in tensors:
         if tensor is not None and tensor.get_device() != device:
-            raise KernelError(f"{name}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
+            _refuse(name, f"a tensor lies on device {tensor.get_device()}, the current device is {device}")
 
 
 def _int4_pages(name: str, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
     """(pages, key/value heads, page size, head size) of a 4-bit cache's four tensors."""
-    _want(name, k_codes.dim() == 4 and k_codes.dtype == torch.uint8 and v_codes.dtype == torch.uint8 and v_codes.shape == k_codes.shape,
-          "codes are uint8 [pages, key/value heads, page size, head size / 2]")
-    pages, n_kv, page_size, half = k_codes.shape
-    _want(name, half in (32, 64), f"head size {2 * half} is not supported in 4 bits (64 and 128 are)")
-    _want(name, k_scales.dtype == v_scales.dtype == torch.bfloat16 and k_scales.shape == v_scales.shape == (pages, n_kv, page_size, 2),
-          "scales are bfloat16 [pages, key/value heads, page size, 2]")
-    _want(name, k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous(),
-          "the cache's tensors are contiguous")
+    shape = k_codes.shape
+    if len(shape) != 4 or k_codes.dtype is not _U8 or v_codes.dtype is not _U8 or v_codes.shape != shape:
+        _refuse(name, "codes are uint8 [pages, key/value heads, page size, head size / 2]")
+    pages, n_kv, page_size, half = shape
+    if half != 64 and half != 32:
+        _refuse(name, f"head size {2 * half} is not supported in 4 bits (64 and 128 are)")
+    shape = (pages, n_kv, page_size, 2)
+    if k_scales.dtype is not _BF16 or v_scales.dtype is not _BF16 or k_scales.shape != shape or v_scales.shape != shape:
+        _refuse(name, "scales are bfloat16 [pages, key/value heads, page size, 2]")
+    if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        _refuse(name, "the cache's tensors are contiguous")
     return pages, n_kv, page_size, 2 * half
 
 
 def _indices(name: str, tensor: torch.Tensor, least: int, what: str) -> None:
-    _want(name, tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous() and tensor.shape[0] >= least, what)
+    """int32, one-dimensional, contiguous, ``least`` of them or more."""
+    if tensor.dtype is not _I32 or tensor.ndim != 1 or tensor.shape[0] < least or not tensor.is_contiguous():
+        _refuse(name, what)
 
 
 def rope_kv_write_int4(qkv: torch.Tensor, bias: torch.Tensor | None, positions: torch.Tensor, slot_mapping: torch.Tensor,
@@ -2134,27 +2141,39 @@ def rope_kv_write_int4(qkv: torch.Tensor, bias: torch.Tensor | None, positions: 
     are not cached; two rows of a step have different slots."""
     name = "rope_kv_write_int4"
     width = (n_q + 2 * n_kv) * head_dim
-    _want(name, qkv.dim() in (2, 3) and qkv.shape[-1] == width and qkv.stride(-1) == 1, f"projections have rows of {width} values")
-    tokens = qkv.shape[-2]
-    if qkv.dim() == 3:
-        _want(name, qkv.dtype == torch.float32 and qkv.is_contiguous(), "partial sums are contiguous float32")
-        n_partials, stride, row_stride = qkv.shape[0], tokens * width, width
-    else:
-        n_partials, stride, row_stride = 1, 0, qkv.stride(0) if tokens > 1 else width
+    shape, strides = qkv.shape, qkv.stride()
+    if len(shape) not in (2, 3) or shape[-1] != width or strides[-1] != 1:
+        _refuse(name, f"projections have rows of {width} values")
+    tokens, n_partials, stride, row_stride = shape[-2], 1, 0, strides[0]
+    if len(shape) == 3:
+        if qkv.dtype is not _FLOAT or not qkv.is_contiguous():
+            _refuse(name, "partial sums are contiguous float32")
+        n_partials, stride, row_stride = shape[0], tokens * width, width
+    elif tokens == 1:
+        row_stride = width
     code = dtype_code(qkv.dtype)
     pages, heads, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
-    _want(name, heads == n_kv and dim == head_dim, f"the cache has {heads} heads of {dim}, the projections {n_kv} of {head_dim}")
+    if heads != n_kv or dim != head_dim:
+        _refuse(name, f"the cache has {heads} heads of {dim}, the projections {n_kv} of {head_dim}")
     _indices(name, positions, tokens, "positions are int32, one a row")
     _indices(name, slot_mapping, tokens, "slots are int32, one a row")
-    _want(name, inv_freq.dtype == torch.float32 and inv_freq.shape == (head_dim // 2,) and inv_freq.is_contiguous(), "frequencies are float32 [head size / 2]")
-    _want(name, q_out.dtype == torch.bfloat16 and q_out.shape == (tokens, n_q, head_dim) and q_out.is_contiguous(),
-          "q_out is contiguous bfloat16 [rows, query heads, head size]")
-    _want(name, bias is None or (bias.dtype == torch.float32 and bias.shape == (width,) and bias.is_contiguous()), f"the bias is float32 [{width}]")
-    _here(name, qkv, bias, positions, slot_mapping, inv_freq, q_out, k_codes, k_scales, v_codes, v_scales)
+    if inv_freq.dtype is not _FLOAT or inv_freq.shape != (head_dim // 2,) or not inv_freq.is_contiguous():
+        _refuse(name, "frequencies are float32 [head size / 2]")
+    if q_out.dtype is not _BF16 or q_out.shape != (tokens, n_q, head_dim) or not q_out.is_contiguous():
+        _refuse(name, "q_out is contiguous bfloat16 [rows, query heads, head size]")
+    if bias is not None and (bias.dtype is not _FLOAT or bias.shape != (width,) or not bias.is_contiguous()):
+        _refuse(name, f"the bias is float32 [{width}]")
+    if not qkv.is_cuda:
+        _need_cuda(qkv)
+    device = _get_device()
+    if not (qkv.get_device() == positions.get_device() == slot_mapping.get_device() == inv_freq.get_device() == q_out.get_device()
+            == k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device() == device
+            and (bias is None or bias.get_device() == device)):
+        _elsewhere(name, device, qkv, bias, positions, slot_mapping, inv_freq, q_out, k_codes, k_scales, v_codes, v_scales)
     check(library.load().lse_rope_kv_write_int4(qkv.data_ptr(), code, n_partials, stride, _ptr(bias), positions.data_ptr(),
                                                 slot_mapping.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(),
                                                 k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), tokens, n_q, n_kv,
-                                                head_dim, page_size, pairing, row_stride, pages, _stream()), name)
+                                                head_dim, page_size, pairing, row_stride, pages, _current_stream(device)), name)
 
 
 def kv_read_int4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
@@ -2163,64 +2182,92 @@ def kv_read_int4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.T
     name = "kv_read_int4"
     pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
     tokens = k_out.shape[0]
-    for out in (k_out, v_out):
-        _want(name, out.dtype == torch.bfloat16 and out.shape == (tokens, n_kv, dim) and out.is_contiguous(),
-              f"outputs are contiguous bfloat16 [rows, {n_kv}, {dim}]")
+    shape = (tokens, n_kv, dim)
+    if (k_out.dtype is not _BF16 or v_out.dtype is not _BF16 or k_out.shape != shape or v_out.shape != shape
+            or not k_out.is_contiguous() or not v_out.is_contiguous()):
+        _refuse(name, f"outputs are contiguous bfloat16 [rows, {n_kv}, {dim}]")
     _indices(name, slot_mapping, tokens, "slots are int32, one a row")
-    _here(name, k_codes, k_scales, v_codes, v_scales, slot_mapping, k_out, v_out)
+    if not k_codes.is_cuda:
+        _need_cuda(k_codes)
+    device = _get_device()
+    if not (k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device() == slot_mapping.get_device()
+            == k_out.get_device() == v_out.get_device() == device):
+        _elsewhere(name, device, k_codes, k_scales, v_codes, v_scales, slot_mapping, k_out, v_out)
     check(library.load().lse_kv_read_int4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
                                           slot_mapping.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), tokens, n_kv, dim, page_size,
-                                          pages, _stream()), name)
+                                          pages, _current_stream(device)), name)
 
 
-def _int4_queries(name: str, q: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor, n_kv: int, dim: int, scale: float) -> None:
-    _want(name, q.dim() == 3 and q.dtype == out.dtype == torch.bfloat16 and out.shape == q.shape, "queries and outputs are bfloat16 [rows, heads, head size]")
-    _want(name, q.is_contiguous() and out.is_contiguous(), "queries and outputs are contiguous")
-    _want(name, q.shape[2] == dim and q.shape[1] % n_kv == 0, f"{q.shape[1]} query heads of {q.shape[2]} do not fit {n_kv} key/value heads of {dim}")
-    _want(name, block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.stride(1) == 1, "block tables are int32 [requests, pages]")
-    _want(name, scale > 0.0, "the scale is positive")
+def _int4_queries(name: str, q: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor, n_kv: int, dim: int, scale: float):
+    """(rows, query heads, requests, width of the block tables, distance between their rows)."""
+    shape = q.shape
+    if len(shape) != 3 or q.dtype is not _BF16 or out.dtype is not _BF16 or out.shape != shape:
+        _refuse(name, "queries and outputs are bfloat16 [rows, heads, head size]")
+    if not q.is_contiguous() or not out.is_contiguous():
+        _refuse(name, "queries and outputs are contiguous")
+    tokens, n_q, size = shape
+    if size != dim or n_q % n_kv:
+        _refuse(name, f"{n_q} query heads of {size} do not fit {n_kv} key/value heads of {dim}")
+    shape, strides = block_tables.shape, block_tables.stride()
+    if block_tables.dtype is not _I32 or len(shape) != 2 or strides[1] != 1:
+        _refuse(name, "block tables are int32 [requests, pages]")
+    if not scale > 0.0:
+        _refuse(name, "the scale is positive")
+    return tokens, n_q, shape[0], shape[1], strides[0]
 
 
 INT4_DECODE_BLOCKS = 4          # blocks that an SM holds
 INT4_DECODE_KEYS = 64           # keys of a part: a tile for each of a block's warps
-INT4_DECODE_CLUSTER = 8         # parts that one launch adds up; more take a second launch
+INT4_DECODE_CLUSTER = 8         # most blocks that share a row's keys in one launch
+INT4_DECODE_RUN_TILES = 8
 
 
-def decode_splits_int4(tokens: int, n_q: int, n_kv: int, max_context: int) -> int:
-    """How many parts the keys of a row are cut into: blocks for all SMs, a tile for each of their warps at least."""
+def decode_parts_int4(tokens: int, n_q: int, n_kv: int, max_context: int) -> tuple[int, int]:
+    """(splits, runs) of a launch: with few tiles of 16 keys, blocks that share a row's keys and add up in one launch (runs 0); with
+    more, all rows' tiles cut into equal runs, a block each, and a second launch for the rows that several blocks had."""
     base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
-    splits = max(1, min(sm_count() * INT4_DECODE_BLOCKS // base, -(-max_context // INT4_DECODE_KEYS)))
-    return splits
+    blocks = sm_count() * INT4_DECODE_BLOCKS
+    tiles = base * -(-max_context // 16)
+    if tiles > INT4_DECODE_RUN_TILES * blocks:
+        return 1, blocks
+    wanted = min(INT4_DECODE_CLUSTER, blocks // base, -(-max_context // INT4_DECODE_KEYS))
+    return 1 << (max(1, wanted).bit_length() - 1), 0
 
 
 def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                                 v_scales: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor,
                                 segment_of_token: torch.Tensor, positions: torch.Tensor, scale: float, max_context: int = 0,
-                                num_splits: int | None = None) -> torch.Tensor:
+                                num_splits: int | None = None, num_runs: int | None = None) -> torch.Tensor:
     """:func:`paged_attention_decode` over a 4-bit cache: every row of q (bfloat16 [T, n_q, D], D 64 or 128) attends to the keys
     0 .. its position of its request.  Rows of segment -1 are left alone; a row at position -1 sees nothing and gets zeros.
     ``max_context``: keys that any request holds at most (0: what the block tables have room for); it and the number of rows decide
-    into how many parts (``num_splits``) the keys are cut."""
+    how the keys are shared among blocks (:func:`decode_parts_int4`), unless ``num_splits`` (blocks a row: up to 8, beyond that as many
+    runs) or ``num_runs`` says so."""
     name = "paged_attention_decode_int4"
     pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
-    _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
-    tokens, n_q, _ = q.shape
+    tokens, n_q, requests, width, table_stride = _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
     _indices(name, segment_of_token, tokens, "segments are int32, one a row")
     _indices(name, positions, tokens, "positions are int32, one a row")
-    _here(name, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_of_token, positions)
+    if not q.is_cuda:
+        _need_cuda(q)
+    device = _get_device()
+    if not (q.get_device() == k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device()
+            == out.get_device() == block_tables.get_device() == segment_of_token.get_device() == positions.get_device() == device):
+        _elsewhere(name, device, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_of_token, positions)
     if tokens == 0:
         return out
-    room = block_tables.shape[1] * page_size
-    if num_splits is None:
-        num_splits = decode_splits_int4(tokens, n_q, n_kv, min(room, max_context) if max_context > 0 else room)
-    scratch = None
-    if num_splits > INT4_DECODE_CLUSTER:
-        scratch = torch.empty(tokens * n_q * num_splits * (dim + 2), dtype=torch.float32, device=q.device)
+    room = width * page_size
+    if num_runs is None and num_splits is None:
+        num_splits, num_runs = decode_parts_int4(tokens, n_q, n_kv, max_context if 0 < max_context < room else room)
+    elif num_runs is None:
+        base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
+        num_splits, num_runs = (1 << (num_splits - 1).bit_length(), 0) if num_splits <= INT4_DECODE_CLUSTER else (1, base * num_splits)
+    scratch = torch.empty(16 * num_runs * (dim + 2), dtype=_FLOAT, device=q.device) if num_runs else None
     check(library.load().lse_paged_attention_decode_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                                          v_scales.data_ptr(), out.data_ptr(), _ptr(scratch), block_tables.data_ptr(),
-                                                         block_tables.stride(0), segment_of_token.data_ptr(), positions.data_ptr(),
-                                                         tokens, n_q, n_kv, dim, page_size, scale, num_splits, pages,
-                                                         block_tables.shape[0], _stream()), name)
+                                                         table_stride, segment_of_token.data_ptr(), positions.data_ptr(), tokens, n_q,
+                                                         n_kv, dim, page_size, scale, num_splits or 1, num_runs, pages, requests,
+                                                         _current_stream(device)), name)
     return out
 
 
@@ -2241,18 +2288,23 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     :func:`paged_attention_decode_int4`; ``max_portions`` (with it): at most so many requests have more."""
     name = "paged_attention_prefill_int4"
     pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
-    _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
-    tokens, n_q, _ = q.shape
-    segments = block_tables.shape[0]
+    tokens, n_q, segments, width, table_stride = _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
     group = n_q // n_kv
-    _want(name, group <= INT4_TILE, f"{group} query heads a key/value head: at most {INT4_TILE}")
-    _want(name, segments > 0, "block tables have a row a request")
+    if group > INT4_TILE:
+        _refuse(name, f"{group} query heads a key/value head: at most {INT4_TILE}")
+    if segments == 0:
+        _refuse(name, "block tables have a row a request")
     _indices(name, segment_start, segments + 1, "segment starts are int32, one more than the requests")
     _indices(name, segment_first_position, segments, "first positions are int32, one a request")
-    _here(name, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_start, segment_first_position)
+    if not q.is_cuda:
+        _need_cuda(q)
+    device = _get_device()
+    if not (q.get_device() == k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device()
+            == out.get_device() == block_tables.get_device() == segment_start.get_device() == segment_first_position.get_device() == device):
+        _elsewhere(name, device, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_start, segment_first_position)
     if tokens == 0:
         return out
-    room = segments * -(-block_tables.shape[1] * page_size // INT4_TILE)
+    room = segments * -(-width * page_size // INT4_TILE)
     capacity = min(room, keys // INT4_TILE + segments) if keys > 0 else room
     a_head = capacity * INT4_TILE * dim
     heads_at_once = min(n_kv, max(1, INT4_WORKSPACE_BYTES // (4 * a_head)))
@@ -2260,15 +2312,16 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     # several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs
     blocks = (-(-tokens // (INT4_TILE // group)) + with_tiles) * heads_at_once
     parts = max(1, min(8, 5 * sm_count() // (4 * blocks)))
-    workspace = torch.empty(2 * heads_at_once * a_head, dtype=torch.float16, device=q.device)
-    scratch = torch.empty(tokens * n_q * parts * (dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+    # float16 keys, float16 values, and (several parts) float32 outputs, maxima and sums of every part
+    halves = heads_at_once * a_head
+    workspace = torch.empty(4 * halves + (4 * tokens * n_q * parts * (dim + 2) if parts > 1 else 0), dtype=_U8, device=q.device)
     at = workspace.data_ptr()
     check(library.load().lse_paged_attention_prefill_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                                                          v_scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(),
-                                                          block_tables.stride(0), segment_start.data_ptr(),
-                                                          segment_first_position.data_ptr(), segments, tokens, pages, n_q, n_kv, dim,
-                                                          page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts,
-                                                          at, at + 2 * heads_at_once * a_head, _ptr(scratch), _stream()), name)
+                                                          v_scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), table_stride,
+                                                          segment_start.data_ptr(), segment_first_position.data_ptr(), segments,
+                                                          tokens, pages, n_q, n_kv, dim, page_size, scale, skip_single, with_tiles,
+                                                          capacity, heads_at_once, parts, at, at + 2 * halves,
+                                                          at + 4 * halves if parts > 1 else None, _current_stream(device)), name)
     return out
 
 
@@ -2286,25 +2339,41 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, ended: torch.Tensor,
     float32, tokens, parents (the beam within the request) and ended (int32: the parent had ended or the token is ``end_token``).
     Where fewer than K are offered the rest are (-inf, end_token, their own number, 1)."""
     name = "beam_select"
-    _want(name, scores.dim() == 2 and scores.dtype == torch.float32, "scores are float32 [requests, beams]")
-    requests, beams = scores.shape
-    _want(name, 1 <= beams <= MAX_BEAMS, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
-    _want(name, logits.dim() == 2 and logits.dtype == torch.float32 and logits.shape[0] == requests * beams and logits.shape[1] > 0
-          and logits.stride(1) == 1, "logits are float32 [requests * beams, vocabulary]")
-    vocab = logits.shape[1]
-    _want(name, 0 <= end_token < vocab, f"the end token {end_token} lies outside the vocabulary")
-    for tensor, kind in ((scores, torch.float32), (ended, torch.int32), (out_scores, torch.float32), (out_tokens, torch.int32),
-                         (out_parents, torch.int32), (out_ended, torch.int32)):
-        _want(name, tensor.dtype == kind and tensor.shape == (requests, beams) and tensor.is_contiguous(),
-              "scores are contiguous float32, the other arrays int32, all [requests, beams]")
-    _here(name, logits, scores, ended, out_scores, out_tokens, out_parents, out_ended)
+    shape = scores.shape
+    if len(shape) != 2 or scores.dtype is not _FLOAT:
+        _refuse(name, "scores are float32 [requests, beams]")
+    requests, beams = shape
+    if not 1 <= beams <= MAX_BEAMS:
+        _refuse(name, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
+    wide, strides = logits.shape, logits.stride()
+    if len(wide) != 2 or logits.dtype is not _FLOAT or wide[0] != requests * beams or wide[1] == 0 or strides[1] != 1:
+        _refuse(name, "logits are float32 [requests * beams, vocabulary]")
+    vocab = wide[1]
+    if not 0 <= end_token < vocab:
+        _refuse(name, f"the end token {end_token} lies outside the vocabulary")
+    if not (ended.dtype is out_tokens.dtype is out_parents.dtype is out_ended.dtype is _I32 and out_scores.dtype is _FLOAT
+            and ended.shape == out_scores.shape == out_tokens.shape == out_parents.shape == out_ended.shape == shape
+            and scores.is_contiguous() and ended.is_contiguous() and out_scores.is_contiguous() and out_tokens.is_contiguous()
+            and out_parents.is_contiguous() and out_ended.is_contiguous()):
+        _refuse(name, "scores are contiguous float32, the other arrays int32, all [requests, beams]")
+    if not logits.is_cuda:
+        _need_cuda(logits)
+    device = _get_device()
+    if not (logits.get_device() == scores.get_device() == ended.get_device() == out_scores.get_device() == out_tokens.get_device()
+            == out_parents.get_device() == out_ended.get_device() == device):
+        _elsewhere(name, device, logits, scores, ended, out_scores, out_tokens, out_parents, out_ended)
     if requests == 0:
         return
     lib = library.load()
-    scratch = torch.empty(1024 * lib.lse_beam_select_scratch_kb(requests, beams, vocab), dtype=torch.uint8, device=logits.device)
-    check(lib.lse_beam_select(logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, requests, beams, vocab,
-                              scores.data_ptr(), ended.data_ptr(), end_token, scratch.data_ptr(), out_scores.data_ptr(),
-                              out_tokens.data_ptr(), out_parents.data_ptr(), out_ended.data_ptr(), _stream()), name)
+    scratch = torch.empty(_beam_scratch(requests, beams, vocab), dtype=_U8, device=logits.device)
+    check(lib.lse_beam_select(logits.data_ptr(), strides[0] if wide[0] > 1 else vocab, requests, beams, vocab, scores.data_ptr(),
+                              ended.data_ptr(), end_token, scratch.data_ptr(), out_scores.data_ptr(), out_tokens.data_ptr(),
+                              out_parents.data_ptr(), out_ended.data_ptr(), _current_stream(device)), name)
+
+
+@functools.lru_cache(maxsize=256)
+def _beam_scratch(requests: int, beams: int, vocab: int) -> int:
+    return 1024 * int(library.load().lse_beam_select_scratch_kb(requests, beams, vocab))      # follows from the sizes alone
 
 
 MAX_REORDER_STORAGES = 24
@@ -2321,31 +2390,55 @@ def beam_reorder(parents: torch.Tensor, block_tables: torch.Tensor, lengths: tor
     contiguous (a group's storage as [layers * 2, pages, ...]; states as [1, slots, ...] with tables of one column, lengths of
     1 and a page size of 2).  A page that is being filled belongs to one beam only."""
     name = "beam_reorder"
-    _want(name, parents.dim() == 2 and parents.dtype == torch.int32 and parents.is_contiguous(), "parents are int32 [requests, beams]")
-    requests, beams = parents.shape
-    _want(name, 1 <= beams <= MAX_BEAMS, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
-    _want(name, page_size > 0, "the page size is positive")
-    for tables in (block_tables, new_tables):
-        _want(name, tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == requests * beams and tables.shape[1] > 0
-              and tables.stride(1) == 1 and tables.shape == block_tables.shape, "block tables are int32 [requests * beams, pages]")
-    _want(name, new_tables.data_ptr() != block_tables.data_ptr(), "the new tables are made in another tensor than the old ones")
+    shape = parents.shape
+    if len(shape) != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
+        _refuse(name, "parents are int32 [requests, beams]")
+    requests, beams = shape
+    if not 1 <= beams <= MAX_BEAMS:
+        _refuse(name, f"{beams} beams: 1 to {MAX_BEAMS} are supported")
+    if page_size <= 0:
+        _refuse(name, "the page size is positive")
+    shape, strides, new_strides = block_tables.shape, block_tables.stride(), new_tables.stride()
+    if (len(shape) != 2 or block_tables.dtype is not _I32 or new_tables.dtype is not _I32 or shape[0] != requests * beams or shape[1] == 0
+            or new_tables.shape != shape or strides[1] != 1 or new_strides[1] != 1):
+        _refuse(name, "block tables are int32 [requests * beams, pages]")
+    tables_at, new_at = block_tables.data_ptr(), new_tables.data_ptr()
+    if tables_at == new_at:
+        _refuse(name, "the new tables are made in another tensor than the old ones")
     _indices(name, lengths, requests, "lengths are int32, one a request")
-    numbers = []
+    numbers, where = [], set()
     for storage in storages:
-        _want(name, storage.dim() >= 3 and storage[0, 0].is_contiguous(), "storages are [outer, pages, ...] with contiguous pages")
-        size = storage.element_size()
-        numbers.append((storage.data_ptr(), storage.shape[0], storage.stride(0) * size, storage.stride(1) * size,
-                        storage[0, 0].numel() * size, storage.shape[1]))
-    _here(name, parents, block_tables, lengths, new_tables, *storages)
+        numbers += _storage_numbers(name, storage)
+        where.add(storage.get_device())
+    if not parents.is_cuda:
+        _need_cuda(parents)
+    device = _get_device()
+    if (not parents.get_device() == block_tables.get_device() == lengths.get_device() == new_tables.get_device() == device
+            or not where <= {device}):
+        _elsewhere(name, device, parents, block_tables, lengths, new_tables, *storages)
     if requests == 0:
         return
-    lib = library.load()
-    for at in range(0, max(1, len(numbers)), MAX_REORDER_STORAGES):
-        some = numbers[at:at + MAX_REORDER_STORAGES]
-        flat = (c_longlong * (6 * max(1, len(some))))(*(number for storage in some for number in storage))
-        check(lib.lse_beam_reorder(parents.data_ptr(), requests, beams, block_tables.data_ptr(), block_tables.stride(0),
-                                   block_tables.shape[1], lengths.data_ptr(), page_size, new_tables.data_ptr() if at == 0 else None,
-                                   new_tables.stride(0), flat, len(some), _stream()), name)
+    lib, stream = library.load(), _current_stream(device)
+    for at in range(0, max(1, len(storages)), MAX_REORDER_STORAGES):
+        some = numbers[6 * at:6 * (at + MAX_REORDER_STORAGES)]
+        check(lib.lse_beam_reorder(parents.data_ptr(), requests, beams, tables_at, strides[0], shape[1], lengths.data_ptr(), page_size,
+                                   new_at if at == 0 else None, new_strides[0], (c_longlong * max(6, len(some)))(*some),
+                                   len(some) // 6, stream), name)
+
+
+def _storage_numbers(name: str, storage: torch.Tensor) -> tuple:
+    """Address, outer parts, bytes between them, bytes between pages, bytes of a page, pages."""
+    shape, strides, size = storage.shape, storage.stride(), storage.element_size()
+    if len(shape) < 3 or 0 in shape:
+        _refuse(name, "storages are [outer, pages, ...] with contiguous pages")
+    a_page = storage.numel() // (shape[0] * shape[1])
+    if not storage.is_contiguous():
+        inner = 1
+        for n, stride in zip(shape[:1:-1], strides[:1:-1]):
+            if n != 1 and stride != inner:
+                _refuse(name, "storages are [outer, pages, ...] with contiguous pages")
+            inner *= n
+    return storage.data_ptr(), shape[0], strides[0] * size, strides[1] * size, a_page * size, shape[1]
 
 
 def step_tables(first: torch.Tensor, counts: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, page_size: int,
@@ -2357,22 +2450,38 @@ def step_tables(first: torch.Tensor, counts: torch.Tensor, pages: torch.Tensor, 
     (all int32).  Written (int32): segment_start [S + 1], segment_of_token, positions and slot_mapping [T] (rows behind the last
     request: -1, 0, -1; a row whose page is missing or -1: slot -1), contexts [S], block_tables [S, W] (-1 behind a request's pages)."""
     name = "step_tables"
-    _indices(name, first, 1, "first positions are int32, one a request")
-    requests = first.shape[0]
-    _indices(name, counts, requests, "counts are int32, one a request")
-    _indices(name, page_start, requests + 1, "page starts are int32, one more than the requests")
-    _indices(name, pages, 0, "pages are int32")
-    _indices(name, segment_start, requests + 1, "segment starts are int32, one more than the requests")
-    _indices(name, contexts, requests, "contexts are int32, one a request")
-    tokens = segment_of_token.shape[0]
-    for rows in (segment_of_token, positions, slot_mapping):
-        _indices(name, rows, tokens, "segments, positions and slots are int32, one a row")
-    _want(name, page_size > 0, "the page size is positive")
-    _want(name, block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == requests
-          and block_tables.stride(1) == 1, "block tables are int32 [requests, pages]")
-    _here(name, first, counts, pages, page_start, segment_start, segment_of_token, positions, slot_mapping, contexts, block_tables)
-    width = block_tables.shape[1]
+    requests, tokens = first.shape[0], segment_of_token.shape[0]
+    a_row = (1,)
+    if not (first.dtype is counts.dtype is pages.dtype is page_start.dtype is segment_start.dtype is segment_of_token.dtype
+            is positions.dtype is slot_mapping.dtype is contexts.dtype is _I32 and requests > 0
+            and first.stride() == counts.stride() == pages.stride() == page_start.stride() == segment_start.stride()
+            == segment_of_token.stride() == positions.stride() == slot_mapping.stride() == contexts.stride() == a_row
+            and counts.shape[0] >= requests and page_start.shape[0] > requests and segment_start.shape[0] > requests
+            and contexts.shape[0] >= requests and positions.shape[0] >= tokens and slot_mapping.shape[0] >= tokens):
+        # one by one (tensors of one number or none may have strides of their own)
+        _indices(name, first, 1, "first positions are int32, one a request")
+        _indices(name, counts, requests, "counts are int32, one a request")
+        _indices(name, page_start, requests + 1, "page starts are int32, one more than the requests")
+        _indices(name, pages, 0, "pages are int32")
+        _indices(name, segment_start, requests + 1, "segment starts are int32, one more than the requests")
+        _indices(name, contexts, requests, "contexts are int32, one a request")
+        _indices(name, segment_of_token, tokens, "segments, positions and slots are int32, one a row")
+        _indices(name, positions, tokens, "segments, positions and slots are int32, one a row")
+        _indices(name, slot_mapping, tokens, "segments, positions and slots are int32, one a row")
+    if page_size <= 0:
+        _refuse(name, "the page size is positive")
+    shape, strides = block_tables.shape, block_tables.stride()
+    if block_tables.dtype is not _I32 or len(shape) != 2 or shape[0] != requests or strides[1] != 1:
+        _refuse(name, "block tables are int32 [requests, pages]")
+    if not first.is_cuda:
+        _need_cuda(first)
+    device = _get_device()
+    if not (first.get_device() == counts.get_device() == pages.get_device() == page_start.get_device() == segment_start.get_device()
+            == segment_of_token.get_device() == positions.get_device() == slot_mapping.get_device() == contexts.get_device()
+            == block_tables.get_device() == device):
+        _elsewhere(name, device, first, counts, pages, page_start, segment_start, segment_of_token, positions, slot_mapping, contexts, block_tables)
+    width = shape[1]
     check(library.load().lse_step_tables(first.data_ptr(), counts.data_ptr(), pages.data_ptr(), page_start.data_ptr(), requests,
                                          page_size, tokens, segment_start.data_ptr(), segment_of_token.data_ptr(),
                                          positions.data_ptr(), slot_mapping.data_ptr(), contexts.data_ptr(), block_tables.data_ptr(),
-                                         max(width, block_tables.stride(0)), width, _stream()), name)
+                                         max(width, strides[0]), width, _current_stream(device)), name)

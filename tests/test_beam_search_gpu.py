@@ -22,8 +22,16 @@ def compare(logits, scores, ended, end_token):
     got = [t.cpu() for t in choose(logits.cuda() if not logits.is_cuda else logits, scores.cuda(), ended.cuda(), end_token)]
     want = plain.select(logits.cpu(), scores, ended, end_token)
     for r, rows in enumerate(want):
+        assert len({(int(got[1][r, k]), int(got[2][r, k])) for k, row in enumerate(rows) if row[0] > -math.inf}) == sum(row[0] > -math.inf for row in rows)
         for k, (value, token, parent, over) in enumerate(rows):
-            assert (int(got[1][r, k]), int(got[2][r, k]), int(got[3][r, k])) == (token, parent, over), (r, k)
+            there = int(got[1][r, k]), int(got[2][r, k]), int(got[3][r, k])
+            if there != (token, parent, over):
+                # An exponential is off by up to 2^-22 of itself, so a row's lse by as much: offers of two beams that are closer than
+                # twice that may come in either order (offers of one beam share its lse, and may not).
+                assert there[1] != parent and there[2] == int(bool(ended[r, there[1]]) or there[0] == end_token), (r, k)
+                row = logits[r * scores.shape[1] + there[1]].double().cpu()
+                offered = float(scores[r, there[1]]) + (0.0 if ended[r, there[1]] else float(row[there[0]] - torch.logsumexp(row, 0)))
+                assert abs(offered - value) <= 2.0 ** -21, (r, k)
             # one rounding to float32, and the exponentials' (2^-22 each, of a sum of them)
             assert got[0][r, k] == value or abs(float(got[0][r, k]) - value) <= 2.0 ** -24 * abs(value) + 2.0 ** -21
 
@@ -45,6 +53,16 @@ def test_select_of_strided_and_unaligned_rows():
     for start in (0, 1, 2, 3, 5):
         compare(wide[:, start:start + 8190], -torch.rand((3, 4), generator=g), torch.zeros((3, 4), dtype=torch.int32), 0)
         compare(wide[::2, start:start + 2048], -torch.rand((2, 3), generator=g), torch.zeros((2, 3), dtype=torch.int32), 0)
+
+
+def test_equal_rows_make_equal_offers():
+    """Beams that all hold the same prompt: rows that begin at every place relative to a 16-byte boundary, the same to the last bit."""
+    g = torch.Generator().manual_seed(12)
+    row = 3 * torch.randn(70_001, generator=g)
+    logits = row.repeat(8, 1)
+    tokens = torch.topk(row, 1).indices.tolist() * 8
+    got = choose(logits.cuda(), torch.zeros((1, 8)).cuda(), torch.zeros((1, 8), dtype=torch.int32).cuda(), 3)
+    assert got[1][0].tolist() == tokens and got[2][0].tolist() == list(range(8)) and len(set(got[0][0].tolist())) == 1
 
 
 def test_select_of_ties():
@@ -172,3 +190,13 @@ def test_step_tables_of_no_rows():
     start, contexts, tables = ints(5, 5, 5), ints(5, 5), torch.full((2, 2), 5, dtype=torch.int32, device="cuda")
     ops.step_tables(ints(3, 4), ints(0, 0), ints(8, 9), ints(0, 1, 2), 16, start, none, none.clone(), none.clone(), contexts, tables)
     assert start.tolist() == [0, 0, 0] and contexts.tolist() == [3, 4] and tables.tolist() == [[8, -1], [9, -1]]
+
+
+def test_select_of_logits_far_below_zero():
+    """A vocabulary of which parts are ruled out, the rest far below zero: sums of exponentials that only powers of two keep apart."""
+    logits = torch.full((4, 9000), -math.inf)
+    logits[0, 5000:5100] = -20_000.0 + torch.arange(100.0)
+    logits[1, ::3] = 30_000.0 - torch.arange(3000.0)
+    logits[2, 8999] = -3e38
+    logits[3, :] = -1000.0
+    compare(logits, torch.zeros((2, 2)), torch.zeros((2, 2), dtype=torch.int32), 0)
