@@ -5,7 +5,7 @@
 // score, the scale of a value its probability, and c costs one multiply-add a score.  (Making values of the codes first would
 // round them to bfloat16 and cost a multiply-add a value.)
 //
-// One block = (row, up to 8 query heads of a key/value head, a part of the keys); its warps take tiles of 32 keys in turn.  Keys ride the
+// One block = (row, up to 8 query heads of a key/value head, a part of the keys); its warps take tiles of 16 keys in turn.  Keys ride the
 // M side of mma.sync m16n8k16, heads the N side (S^T = K Q^T, O^T = V^T P^T).  Codes go from global memory straight into the
 // registers that the instruction wants them in: which d a thread holds where is free as long as q, or the output, follows, so
 //   keys    lane 4 g + t reads D / 8 consecutive bytes of keys g and g + 8: its d are t D / 4 .. ;
@@ -28,12 +28,12 @@ LSE_CHECK_DEFINE(lse_check_attention_int4)
 
 namespace {
 
-constexpr int SIDE = 16, SIDES = 2, TILE = SIDE * SIDES;     // keys a warp takes at a time: SIDES times the instruction's M side
+constexpr int SIDE = 16, SIDES = 1, TILE = SIDE * SIDES;     // keys a warp takes at a time: SIDES times the instruction's M side
 constexpr int HEADS = 8;         // query heads of a group that a block takes: the N side of the instruction
 constexpr int WARPS = 4, BLOCKS = 4;     // warps of a block, blocks of an SM
-constexpr int STAGE = 128;       // tiles whose places a block keeps in shared memory at a time
+constexpr int STAGE = 256;       // tiles whose places a block keeps in shared memory at a time
 constexpr int MAX_CLUSTER = 8;   // parts that are added up through distributed shared memory
-constexpr int STAGES = 3;        // tiles of a warp that are on their way or worked on
+constexpr int STAGES = 4;        // tiles of a warp that are on their way or worked on
 constexpr float RAISE = 8.0f;    // in powers of two
 
 // Nibbles at bits 4 N of each half of x as two bfloat16: 16 + u (a shift to the mantissa's upper bits and one and-or; 24 too much,
@@ -473,8 +473,9 @@ __device__ __forceinline__ unsigned walk_rows(const int* __restrict__ segment_of
 template <int D, int UNIT>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
 attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, __nv_bfloat16* __restrict__ out, float4* __restrict__ part_o,
-                      float2* __restrict__ part_ml, const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_of_token,
-                      const int* __restrict__ positions, int tokens, int n_q, float scale_log2e, int group, int gchunks, int num_segments) {
+                      float2* __restrict__ part_ml, int2* __restrict__ shares, const int* __restrict__ block_tables, int bt_stride,
+                      const int* __restrict__ segment_of_token, const int* __restrict__ positions, int tokens, int n_q, float scale_log2e, int group,
+                      int gchunks, int num_segments) {
   constexpr int THREADS = WARPS * 32;
   extern __shared__ __align__(16) unsigned char smem[];
   Shared4<D, UNIT>& sh = *reinterpret_cast<Shared4<D, UNIT>*>(smem);
@@ -500,6 +501,16 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
   const unsigned inside = begin - start_s[2] * columns;
   unsigned at = begin, column = begin < end ? inside / n : 0;
   int tile = begin < end ? inside - column * n : 0;
+  // A row that sees nothing gets zeros, a padding row nothing at all: the first block's threads, a row each.
+  if (blockIdx.x == 0) {
+    pdl_wait();
+    for (int r = tid; r < tokens; r += THREADS) {
+      if (tiles_of(segment_of_token, positions, r) > 0) continue;
+      for (unsigned k = 0; k < columns; ++k) shares[(size_t)r * columns + k] = make_int2(0, 1);
+      if (segment_of_token[r] >= 0)
+        for (int i = 0; i < n_q * D / 8; ++i) reinterpret_cast<uint4*>(out + (size_t)r * n_q * D)[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
   bool first = true;
   if (begin >= end) pdl_wait();
   while (at < end) {
@@ -513,6 +524,9 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
                           scale_log2e, first);
     first = false;
     const bool whole = tile == 0 && tile_hi == n;
+    // whoever has the first of a row's tiles says how many blocks have some of them
+    if (tile == 0 && tid == 0)
+      shares[(size_t)row * columns + column] = make_int2(blockIdx.x, whole ? 1 : (int)(runs.block_of(at + n - 1) - blockIdx.x) + 1);
     const size_t slot = 2 * (size_t)blockIdx.x + (tile == 0 ? 1 : 0);
 #pragma unroll
     for (int item = tid; item < 1 << ITEM_BITS<D>; item += THREADS) {
@@ -543,37 +557,23 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
 constexpr int COMBINE_THREADS = 256;
 template <int D, int SLICES>
 __global__ void __launch_bounds__(COMBINE_THREADS)
-combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ segment_of_token,
-                    const int* __restrict__ positions, __nv_bfloat16* __restrict__ out, int tokens, int blocks, int n_q, int group, int gchunks) {
+combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ shares,
+                    __nv_bfloat16* __restrict__ out, int n_q, int group, int gchunks) {
   constexpr int ITEMS = (1 << ITEM_BITS<D>) / SLICES, PARTS_AT_ONCE = COMBINE_THREADS / ITEMS;
   __shared__ float4 sum_o[COMBINE_THREADS];
   __shared__ float sum_m[COMBINE_THREADS], sum_l[COMBINE_THREADS];
-  __shared__ unsigned sums[COMBINE_THREADS / 32], mine_s[2];
   const int row = blockIdx.x, column = blockIdx.y;
-  const unsigned columns = gridDim.y;
   pdl_launch_dependents();
-  const unsigned all = walk_rows<COMBINE_THREADS>(segment_of_token, positions, tokens, sums, [&](int base, unsigned mine, unsigned before) {
-    if (base + (int)threadIdx.x == row) { mine_s[0] = mine; mine_s[1] = before; }
-  });
-  __syncthreads();
-  const unsigned n = mine_s[0], from = mine_s[1] * columns + column * n;
-  const Runs runs(all * columns, blocks);
-  // the blocks whose runs hold the first and the last of the tiles
-  const unsigned b0 = n > 0 ? runs.block_of(from) : 0, b1 = n > 0 ? runs.block_of(from + n - 1) : 0;
   pdl_wait();
-  if (segment_of_token[row] < 0) return;
+  const int2 share = shares[(size_t)row * gridDim.y + column];
+  const int b0 = share.x, parts = share.y;
+  if (parts == 1) return;  // finished there
   const int item = blockIdx.z * ITEMS + threadIdx.x % ITEMS, lane_part = threadIdx.x / ITEMS;
   int h, d;
   item_place<D>(item, h, d);
   const int kvh = column / gchunks, g0 = column % gchunks * HEADS;
   const bool live = h < min(HEADS, group - g0);
   __nv_bfloat16* dst = out + ((size_t)row * n_q + kvh * group + g0 + h) * D + d;
-  if (n == 0) {            // a row that sees nothing
-    if (live && lane_part == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(0u, 0u);
-    return;
-  }
-  const int parts = b1 - b0 + 1;
-  if (parts == 1) return;  // finished there
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int AT_ONCE = 4;       // loads in flight
@@ -629,14 +629,15 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
     if (err != cudaSuccess) return (int)err;
     float4* part_o = reinterpret_cast<float4*>(scratch);
     float2* part_ml = reinterpret_cast<float2*>(scratch + (size_t)2 * runs * HEADS * D);
+    int2* shares = reinterpret_cast<int2*>(part_ml + (size_t)2 * runs * HEADS);
     err = lse_launch(attn_runs_int4_kernel<D, UNIT>, dim3((unsigned)runs), dim3(WARPS * 32), smem, stream, (const __nv_bfloat16*)q, cache,
-                     (__nv_bfloat16*)out, part_o, part_ml, block_tables, bt_stride, segment_of_token, positions, tokens, n_q, scale * LOG2E, group,
-                     gchunks, num_segments);
+                     (__nv_bfloat16*)out, part_o, part_ml, shares, block_tables, bt_stride, segment_of_token, positions, tokens, n_q, scale * LOG2E,
+                     group, gchunks, num_segments);
     if (err != cudaSuccess) return (int)err;
     // more than eight parts a row on average: eight slices, so that the parts of one long row are added up by more than its few blocks
 #define LSE_INT4_COMBINE(SLICES)                                                                                                 \
   lse_launch(combine_runs_kernel<D, SLICES>, dim3((unsigned)tokens, (unsigned)columns, SLICES), dim3(COMBINE_THREADS), 0, stream,       \
-             (const float4*)part_o, (const float2*)part_ml, segment_of_token, positions, (__nv_bfloat16*)out, tokens, runs, n_q, group, gchunks)
+             (const float4*)part_o, (const float2*)part_ml, (const int2*)shares, (__nv_bfloat16*)out, n_q, group, gchunks)
     err = (long long)tokens * columns * 8 < runs ? LSE_INT4_COMBINE(8) : LSE_INT4_COMBINE(1);
 #undef LSE_INT4_COMBINE
   } else {
@@ -661,7 +662,7 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
 // q, out bfloat16 [tokens, n_q, head_dim]; the cache as int4_cache.cu leaves it; block_tables [num_segments, bt_stride].
 // segment_of_token < 0: a padding row, left as it was; a row at a negative position sees no key and gets zeros.
 // runs = 0: a row's keys are shared by `splits` blocks (1, 2, 4 or 8); runs > 0: all rows' tiles are cut into so many equal runs, and `scratch`
-// holds 16 runs (head_dim + 2) float32.
+// holds 16 runs (head_dim + 2) + 2 tokens n_kv ceil(n_q / n_kv / 8) words.
 extern "C" int lse_paged_attention_decode_int4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                                                const void* v_scales, void* out, float* scratch, const int* block_tables,
                                                int bt_stride, const int* segment_of_token, const int* positions, int tokens,

@@ -2217,21 +2217,23 @@ def _int4_queries(name: str, q: torch.Tensor, out: torch.Tensor, block_tables: t
 
 
 INT4_DECODE_BLOCKS = 4          # blocks that an SM holds
-INT4_DECODE_KEYS = 64           # keys of a part: a tile for each of a block's warps
+INT4_DECODE_WARPS = 4           # warps of a block, which take tiles of 16 keys in turn
 INT4_DECODE_CLUSTER = 8         # most blocks that share a row's keys in one launch
-INT4_DECODE_RUN_TILES = 8
+# Tiles of a warp beyond which all rows' tiles are cut into equal runs: with contexts from a half to one and a half times 1,900, 64
+# rows of 12 / 2 heads (11 tiles) take 16.6 us in one launch and 18 to 20 in runs, with 6,000, 16 rows of 8 heads of 64 (35 tiles) 27
+# and 23; one row of 28 / 4 heads over 30,000 keys 31 and 12.
+INT4_DECODE_TILES = 14
 
 
-def decode_parts_int4(tokens: int, n_q: int, n_kv: int, max_context: int) -> tuple[int, int]:
-    """(splits, runs) of a launch: with few tiles of 16 keys, blocks that share a row's keys and add up in one launch (runs 0); with
-    more, all rows' tiles cut into equal runs, a block each, and a second launch for the rows that several blocks had."""
-    base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
-    blocks = sm_count() * INT4_DECODE_BLOCKS
-    tiles = base * -(-max_context // 16)
-    if tiles > INT4_DECODE_RUN_TILES * blocks:
-        return 1, blocks
-    wanted = min(INT4_DECODE_CLUSTER, blocks // base, -(-max_context // INT4_DECODE_KEYS))
-    return 1 << (max(1, wanted).bit_length() - 1), 0
+@functools.lru_cache(maxsize=4096)
+def decode_parts_int4(tokens: int, n_q: int, n_kv: int, max_context: int, multiprocessors: int) -> tuple[int, int]:
+    """(splits, runs) of a launch: with few tiles, blocks that share a row's keys and add up in one launch (runs 0); with many, all
+    rows' tiles cut into equal runs, a block each, and a second launch for the rows that several blocks had."""
+    columns = n_kv * ((n_q // n_kv + 7) // 8)
+    blocks, tiles = multiprocessors * INT4_DECODE_BLOCKS, -(-max_context // 16)
+    wanted = min(INT4_DECODE_CLUSTER, blocks // (tokens * columns), -(-tiles // INT4_DECODE_WARPS))
+    splits = 1 << (max(1, wanted).bit_length() - 1)
+    return (1, blocks) if tiles > INT4_DECODE_TILES * splits * INT4_DECODE_WARPS else (splits, 0)
 
 
 def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
@@ -2258,11 +2260,12 @@ def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
         return out
     room = width * page_size
     if num_runs is None and num_splits is None:
-        num_splits, num_runs = decode_parts_int4(tokens, n_q, n_kv, max_context if 0 < max_context < room else room)
+        num_splits, num_runs = decode_parts_int4(tokens, n_q, n_kv, max_context if 0 < max_context < room else room,
+                                                 _SM_COUNT.get(device) or sm_count())
     elif num_runs is None:
         base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
         num_splits, num_runs = (1 << (num_splits - 1).bit_length(), 0) if num_splits <= INT4_DECODE_CLUSTER else (1, base * num_splits)
-    scratch = torch.empty(16 * num_runs * (dim + 2), dtype=_FLOAT, device=q.device) if num_runs else None
+    scratch = torch.empty(16 * num_runs * (dim + 2) + 2 * tokens * n_q, dtype=_FLOAT, device=q.device) if num_runs else None
     check(library.load().lse_paged_attention_decode_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                                          v_scales.data_ptr(), out.data_ptr(), _ptr(scratch), block_tables.data_ptr(),
                                                          table_stride, segment_of_token.data_ptr(), positions.data_ptr(), tokens, n_q,
