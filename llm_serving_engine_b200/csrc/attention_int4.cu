@@ -352,29 +352,44 @@ __device__ __forceinline__ void store_result(__nv_bfloat16* out, float4 o, float
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
+// Where a launch's rows lie: row r of q at positions[r], of request segment_of_token[r] (negative: a padding row); or (segment_start given:
+// a step that also holds prompt portions) row r is the one token of request r, and requests of other counts have none.
+struct Rows {
+  const int *segment_of_token, *positions, *segment_start;
+  // the token, and its request; a negative request: there is nothing to do
+  __device__ __forceinline__ int find(int r, int& token) const {
+    token = r;
+    if (segment_start != nullptr) {
+      token = segment_start[r];
+      if (segment_start[r + 1] - token != 1) return -1;
+    }
+    return segment_of_token[token];
+  }
+};
+
 // Few tiles: a block for (row, up to 8 heads of a key/value head, part of the keys), grid (rows, n_kv * gchunks, 1 << cshift).  The parts
 // are a thread-block cluster and are added up through distributed shared memory: one launch.
 template <int D, int UNIT, bool CLUSTER>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
 attn_decode_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, __nv_bfloat16* __restrict__ out,
-                        const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_of_token,
-                        const int* __restrict__ positions, int n_q, float scale_log2e, int cshift, int group, int gchunks, int num_segments) {
+                        const int* __restrict__ block_tables, int bt_stride, const Rows rows, int n_q, float scale_log2e, int cshift, int group,
+                        int gchunks, int num_segments) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared4<D, UNIT>& sh = *reinterpret_cast<Shared4<D, UNIT>*>(smem);
   __shared__ float4 recv_o[CLUSTER ? 1 << ITEM_BITS<D> : 1];
   __shared__ float recv_m[MAX_CLUSTER * HEADS], recv_l[MAX_CLUSTER * HEADS];
   pdl_launch_dependents();
   // segments, positions and block tables are the step's own data: read before the wait for the kernels before
-  const int row = blockIdx.x;
+  int token;
   const int kvh = gchunks == 1 ? blockIdx.y : blockIdx.y / gchunks, g0 = gchunks == 1 ? 0 : (blockIdx.y % gchunks) * HEADS;
   const int gcount = min(HEADS, group - g0);
-  const int seg = LSE_CHECKED(segment_of_token[row], -1, num_segments, -1, LSE_CHECK_SEGMENT);
+  const int seg = LSE_CHECKED(rows.find(blockIdx.x, token), -1, num_segments, -1, LSE_CHECK_SEGMENT);
   if (seg < 0) {                   // a padding row (all blocks of its cluster leave together)
     pdl_wait();                    // (a launch without work must not end before the one before it)
     return;
   }
-  const int ctx = positions[row] + 1, csize = 1 << cshift, rank = blockIdx.z, tid = threadIdx.x;
-  const size_t first_head = (size_t)row * n_q + kvh * group + g0;
+  const int ctx = rows.positions[token] + 1, csize = 1 << cshift, rank = blockIdx.z, tid = threadIdx.x;
+  const size_t first_head = (size_t)token * n_q + kvh * group + g0;
   const int total = (max(ctx, 0) + TILE - 1) / TILE, a_part = (total + csize - 1) >> cshift;
   const int tile_lo = min(total, rank * a_part), tile_hi = min(total, tile_lo + a_part);
   cg::cluster_group cluster = cg::this_cluster();
@@ -428,8 +443,9 @@ attn_decode_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache,
 // are blocks, alike but for one tile, whatever the rows' contexts are.  A row's heads whose tiles lie in one block are finished by it;
 // else each block leaves its part (slot 2 b: a part that does not begin at the first key, 2 b + 1: one that does), and
 // combine_runs_kernel adds the parts up.
-__device__ __forceinline__ unsigned tiles_of(const int* __restrict__ segment_of_token, const int* __restrict__ positions, int row) {
-  return segment_of_token[row] >= 0 ? (unsigned)(max(positions[row] + 1, 0) + TILE - 1) / TILE : 0u;
+__device__ __forceinline__ unsigned tiles_of(const Rows& rows, int row) {
+  int token;
+  return rows.find(row, token) >= 0 ? (unsigned)(max(rows.positions[token] + 1, 0) + TILE - 1) / TILE : 0u;
 }
 struct Runs {                  // `work` tiles over `blocks` blocks: the first `longer` of them get one more than the others
   unsigned a_block, longer;
@@ -443,12 +459,11 @@ struct Runs {                  // `work` tiles over `blocks` blocks: the first `
 // Running sums of the rows' tiles by a whole block, as many rows at a time as it has threads: at(base, mine, before) gets every
 // thread's row base + threadIdx.x, its tiles and those of all rows before it.  Returns the sum of all.
 template <int THREADS, typename At>
-__device__ __forceinline__ unsigned walk_rows(const int* __restrict__ segment_of_token, const int* __restrict__ positions, int tokens,
-                                              unsigned (&sums)[THREADS / 32], At at) {
+__device__ __forceinline__ unsigned walk_rows(const Rows& rows, int tokens, unsigned (&sums)[THREADS / 32], At at) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned before = 0;
   for (int base = 0; base < tokens; base += THREADS) {
-    const unsigned mine = base + tid < tokens ? tiles_of(segment_of_token, positions, base + tid) : 0u;
+    const unsigned mine = base + tid < tokens ? tiles_of(rows, base + tid) : 0u;
     unsigned incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -474,8 +489,7 @@ template <int D, int UNIT>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
 attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, __nv_bfloat16* __restrict__ out, float4* __restrict__ part_o,
                       float2* __restrict__ part_ml, int2* __restrict__ shares, const int* __restrict__ block_tables, int bt_stride,
-                      const int* __restrict__ segment_of_token, const int* __restrict__ positions, int tokens, int n_q, float scale_log2e, int group,
-                      int gchunks, int num_segments) {
+                      const Rows rows, int tokens, int n_q, float scale_log2e, int group, int gchunks, int num_segments) {
   constexpr int THREADS = WARPS * 32;
   extern __shared__ __align__(16) unsigned char smem[];
   Shared4<D, UNIT>& sh = *reinterpret_cast<Shared4<D, UNIT>*>(smem);
@@ -484,7 +498,7 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
   const unsigned columns = cache.n_kv * gchunks;
   const int tid = threadIdx.x;
   unsigned mine_0 = 0, before_0 = 0;      // (a launch of up to 128 rows: they are looked at once)
-  const unsigned all = walk_rows<THREADS>(segment_of_token, positions, tokens, sums,
+  const unsigned all = walk_rows<THREADS>(rows, tokens, sums,
                                           [&](int base, unsigned mine, unsigned before) { if (base == 0) { mine_0 = mine; before_0 = before; } });
   const Runs runs(all * columns, gridDim.x);
   const unsigned begin = runs.begin(blockIdx.x), end = runs.begin(blockIdx.x + 1);
@@ -494,7 +508,7 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
       if (begin >= before * columns && begin < (before + mine) * columns) { start_s[0] = base + tid; start_s[1] = mine; start_s[2] = before; }
     };
     if (tokens <= THREADS) look(0, mine_0, before_0);
-    else { __syncthreads(); walk_rows<THREADS>(segment_of_token, positions, tokens, sums, look); }
+    else { __syncthreads(); walk_rows<THREADS>(rows, tokens, sums, look); }
   }
   __syncthreads();
   int row = start_s[0], n = start_s[1];
@@ -505,10 +519,11 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
   if (blockIdx.x == 0) {
     pdl_wait();
     for (int r = tid; r < tokens; r += THREADS) {
-      if (tiles_of(segment_of_token, positions, r) > 0) continue;
+      if (tiles_of(rows, r) > 0) continue;
       for (unsigned k = 0; k < columns; ++k) shares[(size_t)r * columns + k] = make_int2(0, 1);
-      if (segment_of_token[r] >= 0)
-        for (int i = 0; i < n_q * D / 8; ++i) reinterpret_cast<uint4*>(out + (size_t)r * n_q * D)[i] = make_uint4(0, 0, 0, 0);
+      int token;
+      if (rows.find(r, token) >= 0)
+        for (int i = 0; i < n_q * D / 8; ++i) reinterpret_cast<uint4*>(out + (size_t)token * n_q * D)[i] = make_uint4(0, 0, 0, 0);
     }
   }
   bool first = true;
@@ -517,10 +532,11 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
     const int tile_hi = (int)min((unsigned)n, tile + (end - at));
     const int kvh = gchunks == 1 ? column : column / gchunks, g0 = gchunks == 1 ? 0 : (column % gchunks) * HEADS;
     const int gcount = min(HEADS, group - g0);
-    const int seg = LSE_CHECKED(segment_of_token[row], 0, num_segments, 0, LSE_CHECK_SEGMENT);
-    const size_t first_head = (size_t)row * n_q + kvh * group + g0;
+    int token;
+    const int seg = LSE_CHECKED(rows.find(row, token), 0, num_segments, 0, LSE_CHECK_SEGMENT);
+    const size_t first_head = (size_t)token * n_q + kvh * group + g0;
     if (!first) __syncthreads();       // the results of the run before have been read
-    attend_tiles<D, UNIT>(sh, cache, q + first_head * D, gcount, kvh, block_tables + (size_t)seg * bt_stride, positions[row] + 1, tile, tile_hi,
+    attend_tiles<D, UNIT>(sh, cache, q + first_head * D, gcount, kvh, block_tables + (size_t)seg * bt_stride, rows.positions[token] + 1, tile, tile_hi,
                           scale_log2e, first);
     first = false;
     const bool whole = tile == 0 && tile_hi == n;
@@ -547,7 +563,7 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
     tile = 0;
     if (tile_hi == n && ++column == columns) {
       column = 0;
-      do ++row; while (at < end && (n = (int)tiles_of(segment_of_token, positions, row)) == 0);
+      do ++row; while (at < end && (n = (int)tiles_of(rows, row)) == 0);
     }
   }
 }
@@ -558,7 +574,7 @@ constexpr int COMBINE_THREADS = 256;
 template <int D, int SLICES>
 __global__ void __launch_bounds__(COMBINE_THREADS)
 combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ shares,
-                    __nv_bfloat16* __restrict__ out, int n_q, int group, int gchunks) {
+                    const Rows rows, __nv_bfloat16* __restrict__ out, int n_q, int group, int gchunks) {
   constexpr int ITEMS = (1 << ITEM_BITS<D>) / SLICES, PARTS_AT_ONCE = COMBINE_THREADS / ITEMS;
   __shared__ float4 sum_o[COMBINE_THREADS];
   __shared__ float sum_m[COMBINE_THREADS], sum_l[COMBINE_THREADS];
@@ -573,7 +589,9 @@ combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict_
   item_place<D>(item, h, d);
   const int kvh = column / gchunks, g0 = column % gchunks * HEADS;
   const bool live = h < min(HEADS, group - g0);
-  __nv_bfloat16* dst = out + ((size_t)row * n_q + kvh * group + g0 + h) * D + d;
+  int token;
+  rows.find(row, token);
+  __nv_bfloat16* dst = out + ((size_t)token * n_q + kvh * group + g0 + h) * D + d;
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int AT_ONCE = 4;       // loads in flight
@@ -618,8 +636,7 @@ combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict_
 
 template <int D, int UNIT>
 int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, const int* block_tables, int bt_stride,
-                const int* segment_of_token, const int* positions, int tokens, int n_q, float scale, int splits, int runs, int num_segments,
-                cudaStream_t stream) {
+                const Rows& rows, int tokens, int n_q, float scale, int splits, int runs, int num_segments, cudaStream_t stream) {
   const int group = n_q / cache.n_kv, gchunks = (group + HEADS - 1) / HEADS, columns = cache.n_kv * gchunks;
   constexpr size_t smem = sizeof(Shared4<D, UNIT>), limit = smem + 8192;     // (what is static counts towards the 48 KB that need no leave)
   static SmemAllowance allowance[3];
@@ -631,13 +648,13 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
     float2* part_ml = reinterpret_cast<float2*>(scratch + (size_t)2 * runs * HEADS * D);
     int2* shares = reinterpret_cast<int2*>(part_ml + (size_t)2 * runs * HEADS);
     err = lse_launch(attn_runs_int4_kernel<D, UNIT>, dim3((unsigned)runs), dim3(WARPS * 32), smem, stream, (const __nv_bfloat16*)q, cache,
-                     (__nv_bfloat16*)out, part_o, part_ml, shares, block_tables, bt_stride, segment_of_token, positions, tokens, n_q, scale * LOG2E,
+                     (__nv_bfloat16*)out, part_o, part_ml, shares, block_tables, bt_stride, rows, tokens, n_q, scale * LOG2E,
                      group, gchunks, num_segments);
     if (err != cudaSuccess) return (int)err;
     // more than eight parts a row on average: eight slices, so that the parts of one long row are added up by more than its few blocks
 #define LSE_INT4_COMBINE(SLICES)                                                                                                 \
   lse_launch(combine_runs_kernel<D, SLICES>, dim3((unsigned)tokens, (unsigned)columns, SLICES), dim3(COMBINE_THREADS), 0, stream,       \
-             (const float4*)part_o, (const float2*)part_ml, (const int2*)shares, (__nv_bfloat16*)out, n_q, group, gchunks)
+             (const float4*)part_o, (const float2*)part_ml, (const int2*)shares, rows, (__nv_bfloat16*)out, n_q, group, gchunks)
     err = (long long)tokens * columns * 8 < runs ? LSE_INT4_COMBINE(8) : LSE_INT4_COMBINE(1);
 #undef LSE_INT4_COMBINE
   } else {
@@ -648,7 +665,7 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
     if (err != cudaSuccess) return (int)err;
 #define LSE_INT4_ROWS(CLUSTER)                                                                                                   \
   lse_launch_cluster(attn_decode_int4_kernel<D, UNIT, CLUSTER>, grid, dim3(WARPS * 32), smem, stream, 1u << cshift, (const __nv_bfloat16*)q, cache, \
-                     (__nv_bfloat16*)out, block_tables, bt_stride, segment_of_token, positions, n_q, scale * LOG2E, cshift, group, gchunks, \
+                     (__nv_bfloat16*)out, block_tables, bt_stride, rows, n_q, scale * LOG2E, cshift, group, gchunks, \
                      num_segments)
     err = cshift ? LSE_INT4_ROWS(true) : LSE_INT4_ROWS(false);
 #undef LSE_INT4_ROWS
@@ -660,13 +677,15 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
 }  // namespace
 
 // q, out bfloat16 [tokens, n_q, head_dim]; the cache as int4_cache.cu leaves it; block_tables [num_segments, bt_stride].
-// segment_of_token < 0: a padding row, left as it was; a row at a negative position sees no key and gets zeros.
+// segment_of_token < 0: a padding row, left as it was; a row at a negative position sees no key and gets zeros.  segment_start (may be
+// null): `tokens` counts requests, and the rows are those of requests with one token (see Rows).
 // runs = 0: a row's keys are shared by `splits` blocks (1, 2, 4 or 8); runs > 0: all rows' tiles are cut into so many equal runs, and `scratch`
 // holds 16 runs (head_dim + 2) + 2 tokens n_kv ceil(n_q / n_kv / 8) words.
 extern "C" int lse_paged_attention_decode_int4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                                                const void* v_scales, void* out, float* scratch, const int* block_tables,
-                                               int bt_stride, const int* segment_of_token, const int* positions, int tokens,
-                                               int n_q, int n_kv, int head_dim, int page_size, float scale, int splits, int runs,
+                                               int bt_stride, const int* segment_of_token, const int* positions,
+                                               const int* segment_start, int tokens, int n_q, int n_kv, int head_dim, int page_size,
+                                               float scale, int splits, int runs,
                                                long long num_pages, int num_segments, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_q % n_kv || page_size <= 0 || num_pages <= 0 || splits < 1 || runs < 0 ||
@@ -679,7 +698,8 @@ extern "C" int lse_paged_attention_decode_int4(const void* q, const void* k_code
                   {page_size, -1}, n_kv, (int)num_pages};
   if ((page_size & (page_size - 1)) == 0)
     for (cache.pm.shift = 0; 1 << cache.pm.shift < page_size;) ++cache.pm.shift;
-#define LSE_INT4_ARGS q, cache, out, scratch, block_tables, bt_stride, segment_of_token, positions, tokens, n_q, scale, splits, runs, num_segments, stream
+  const Rows rows = {segment_of_token, positions, segment_start};
+#define LSE_INT4_ARGS q, cache, out, scratch, block_tables, bt_stride, rows, tokens, n_q, scale, splits, runs, num_segments, stream
   const int unit = page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 1;
   if (head_dim == 128) return unit == 16 ? launch_rows<128, 16>(LSE_INT4_ARGS) : unit == 8 ? launch_rows<128, 8>(LSE_INT4_ARGS) : launch_rows<128, 1>(LSE_INT4_ARGS);
   return unit == 16 ? launch_rows<64, 16>(LSE_INT4_ARGS) : unit == 8 ? launch_rows<64, 8>(LSE_INT4_ARGS) : launch_rows<64, 1>(LSE_INT4_ARGS);

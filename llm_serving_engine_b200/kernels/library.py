@@ -22,8 +22,8 @@ _SIGNATURES = {
     "lse_kv_read_int4": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                          c_longlong, c_void_p],
     "lse_paged_attention_decode_int4": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_longlong,
-                                        c_int, c_void_p],
+                                        c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                                        c_longlong, c_int, c_void_p],
     "lse_paged_attention_prefill_int4": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                          c_void_p, c_int, c_int, c_longlong, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],

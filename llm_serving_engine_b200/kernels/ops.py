@@ -2239,12 +2239,14 @@ def decode_parts_int4(tokens: int, n_q: int, n_kv: int, max_context: int, multip
 def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                                 v_scales: torch.Tensor, out: torch.Tensor, block_tables: torch.Tensor,
                                 segment_of_token: torch.Tensor, positions: torch.Tensor, scale: float, max_context: int = 0,
-                                num_splits: int | None = None, num_runs: int | None = None) -> torch.Tensor:
+                                num_splits: int | None = None, num_runs: int | None = None,
+                                segment_start: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`paged_attention_decode` over a 4-bit cache: every row of q (bfloat16 [T, n_q, D], D 64 or 128) attends to the keys
     0 .. its position of its request.  Rows of segment -1 are left alone; a row at position -1 sees nothing and gets zeros.
     ``max_context``: keys that any request holds at most (0: what the block tables have room for); it and the number of rows decide
     how the keys are shared among blocks (:func:`decode_parts_int4`), unless ``num_splits`` (blocks a row: up to 8, beyond that as many
-    runs) or ``num_runs`` says so."""
+    runs) or ``num_runs`` says so.  With ``segment_start`` (int32 [S + 1], a step that also holds prompt portions) the rows are those of
+    the requests that bring exactly one token, and the other rows of ``out`` are left alone."""
     name = "paged_attention_decode_int4"
     pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
     tokens, n_q, requests, width, table_stride = _int4_queries(name, q, out, block_tables, n_kv, dim, scale)
@@ -2256,21 +2258,27 @@ def paged_attention_decode_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     if not (q.get_device() == k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device()
             == out.get_device() == block_tables.get_device() == segment_of_token.get_device() == positions.get_device() == device):
         _elsewhere(name, device, q, k_codes, k_scales, v_codes, v_scales, out, block_tables, segment_of_token, positions)
-    if tokens == 0:
+    if tokens == 0 or requests == 0:
         return out
+    rows = tokens
+    if segment_start is not None:
+        _indices(name, segment_start, requests + 1, "segment starts are int32, one more than the requests")
+        if segment_start.get_device() != device:
+            _elsewhere(name, device, segment_start)
+        rows = requests
     room = width * page_size
     if num_runs is None and num_splits is None:
-        num_splits, num_runs = decode_parts_int4(tokens, n_q, n_kv, max_context if 0 < max_context < room else room,
+        num_splits, num_runs = decode_parts_int4(rows, n_q, n_kv, max_context if 0 < max_context < room else room,
                                                  _SM_COUNT.get(device) or sm_count())
     elif num_runs is None:
-        base = tokens * n_kv * ((n_q // n_kv + 7) // 8)
+        base = rows * n_kv * ((n_q // n_kv + 7) // 8)
         num_splits, num_runs = (1 << (num_splits - 1).bit_length(), 0) if num_splits <= INT4_DECODE_CLUSTER else (1, base * num_splits)
-    scratch = torch.empty(16 * num_runs * (dim + 2) + 2 * tokens * n_q, dtype=_FLOAT, device=q.device) if num_runs else None
+    scratch = torch.empty(16 * num_runs * (dim + 2) + 2 * rows * n_q, dtype=_FLOAT, device=q.device) if num_runs else None
     check(library.load().lse_paged_attention_decode_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                                          v_scales.data_ptr(), out.data_ptr(), _ptr(scratch), block_tables.data_ptr(),
-                                                         table_stride, segment_of_token.data_ptr(), positions.data_ptr(), tokens, n_q,
-                                                         n_kv, dim, page_size, scale, num_splits or 1, num_runs, pages, requests,
-                                                         _current_stream(device)), name)
+                                                         table_stride, segment_of_token.data_ptr(), positions.data_ptr(),
+                                                         _ptr(segment_start), rows, n_q, n_kv, dim, page_size, scale, num_splits or 1,
+                                                         num_runs, pages, requests, _current_stream(device)), name)
     return out
 
 

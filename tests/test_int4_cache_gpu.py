@@ -169,6 +169,25 @@ def test_rows(contexts, n_q, n_kv, dim, page_size, splits):
         assert ((out[row].to(D64) - expected).abs() <= bound(expected, weighed)).all(), (row, s, p)
 
 
+@pytest.mark.parametrize("splits", [1, 4, 9])
+def test_rows_beside_portions(splits):
+    """Requests of one token among portions and empty ones: their rows, wherever these lie, and no other."""
+    counts, firsts = [5, 1, 0, 1, 70, 1], [0, 300, 0, 0, 20, 77]
+    g, cache, tables, start, _ = portion_case(counts, firsts, 2, 64, 16, 6)
+    segments = torch.repeat_interleave(torch.arange(6), torch.tensor(counts)).int().cuda()
+    positions = torch.cat([torch.arange(n) + f for n, f in zip(counts, firsts)]).int().cuda()
+    q = torch.randn((sum(counts), 6, 64), generator=g).bfloat16().cuda()
+    out = torch.full_like(q, 3.0)
+    ops.paged_attention_decode_int4(q, *cache, out, tables, segments, positions, 0.125, num_splits=splits, segment_start=start)
+    for row, (s, p) in enumerate(zip(segments.tolist(), positions.tolist())):
+        if counts[s] != 1:
+            assert (out[row] == 3.0).all()
+            continue
+        k, v = request_rows(cache, tables[s], p + 1, 16)
+        expected, weighed = plain.attend(q[row], k, v, p, 0.125)
+        assert ((out[row].to(D64) - expected).abs() <= bound(expected, weighed)).all()
+
+
 def test_rows_with_scores_far_apart():
     """Maxima that grow from tile to tile by far more than what is put off, and scores of minus and plus a thousand."""
     g = torch.Generator().manual_seed(8)
