@@ -83,7 +83,7 @@ template <int D> __device__ __forceinline__ int value_piece(int i) {     // wher
 // of key/value head kvh: every warp's outputs, maxima and sums are left in `sh`, and the block has met after that.
 // UNIT: keys that certainly lie side by side in the cache (16, 8, or 1: by the page size).
 template <int D, int UNIT>
-__device__ __forceinline__ void attend_tiles(Shared4<D, UNIT>& sh, const Cache4& cache, const __nv_bfloat16* __restrict__ q, int gcount,
+__device__ __forceinline__ void attend_tiles(Shared4<D, UNIT>& sh, const Cache4& cache, const __nv_bfloat16* q, int gcount,
                                              int kvh, const int* __restrict__ bt, int ctx, int tile_lo, int tile_hi, float scale_log2e,
                                              bool wait) {
   constexpr int KW = D / 32, VW = D / 64, TILES_D = D / 16;
@@ -371,7 +371,7 @@ struct Rows {
 // are a thread-block cluster and are added up through distributed shared memory: one launch.
 template <int D, int UNIT, bool CLUSTER>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
-attn_decode_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, __nv_bfloat16* __restrict__ out,
+attn_decode_int4_kernel(const __nv_bfloat16* q, const Cache4 cache, __nv_bfloat16* out,
                         const int* __restrict__ block_tables, int bt_stride, const Rows rows, int n_q, float scale_log2e, int cshift, int group,
                         int gchunks, int num_segments) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -487,8 +487,8 @@ __device__ __forceinline__ unsigned walk_rows(const Rows& rows, int tokens, unsi
 
 template <int D, int UNIT>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
-attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, __nv_bfloat16* __restrict__ out, float4* __restrict__ part_o,
-                      float2* __restrict__ part_ml, int2* __restrict__ shares, const int* __restrict__ block_tables, int bt_stride,
+attn_runs_int4_kernel(const __nv_bfloat16* q, const Cache4 cache, __nv_bfloat16* out, float4* part_o,
+                      float2* part_ml, int2* shares, const int* __restrict__ block_tables, int bt_stride,
                       const Rows rows, int tokens, int n_q, float scale_log2e, int group, int gchunks, int num_segments) {
   constexpr int THREADS = WARPS * 32;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -573,8 +573,8 @@ attn_runs_int4_kernel(const __nv_bfloat16* __restrict__ q, const Cache4 cache, _
 constexpr int COMBINE_THREADS = 256;
 template <int D, int SLICES>
 __global__ void __launch_bounds__(COMBINE_THREADS)
-combine_runs_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ shares,
-                    const Rows rows, __nv_bfloat16* __restrict__ out, int n_q, int group, int gchunks) {
+combine_runs_kernel(const float4* part_o, const float2* part_ml, const int2* shares,
+                    const Rows rows, __nv_bfloat16* out, int n_q, int group, int gchunks) {
   constexpr int ITEMS = (1 << ITEM_BITS<D>) / SLICES, PARTS_AT_ONCE = COMBINE_THREADS / ITEMS;
   __shared__ float4 sum_o[COMBINE_THREADS];
   __shared__ float sum_m[COMBINE_THREADS], sum_l[COMBINE_THREADS];

@@ -80,8 +80,8 @@ __device__ __forceinline__ int tiles_before(const int* __restrict__ segment_star
 constexpr int EXPAND_KEYS = 32;
 template <int D>
 __global__ void __launch_bounds__(256)
-expand_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat162* __restrict__ k_scales,
-                   const unsigned char* __restrict__ v_codes, const __nv_bfloat162* __restrict__ v_scales, uint4* __restrict__ k_out,
+expand_int4_kernel(const unsigned char* k_codes, const __nv_bfloat162* k_scales,
+                   const unsigned char* v_codes, const __nv_bfloat162* v_scales, uint4* __restrict__ k_out,
                    uint4* __restrict__ v_out, const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
                    const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size, int num_pages, int capacity,
                    int skip_single) {
@@ -135,8 +135,8 @@ expand_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat1
       const int logical = (unsigned)key / (unsigned)page_size;
       const int page = LSE_CHECKED(bt[logical], 0, num_pages, 0, LSE_CHECK_TABLE_ENTRY);
       const size_t place = ((size_t)page * n_kv + head0 + head) * page_size + (key - logical * page_size);
-      kx[i] = __ldcs(reinterpret_cast<const uint32_t*>(k_codes + place * (D / 2)) + c);
-      vx[i] = __ldcs(reinterpret_cast<const uint32_t*>(v_codes + place * (D / 2)) + c);
+      kx[i] = reinterpret_cast<const uint32_t*>(k_codes + place * (D / 2))[c];
+      vx[i] = reinterpret_cast<const uint32_t*>(v_codes + place * (D / 2))[c];
       ks[i] = k_scales[place];
       vs[i] = v_scales[place];
     }
@@ -496,7 +496,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 // One block = a tile of rows and a key/value head as attend's, eight (token, head) pairs of it; a warp adds up the parts of a pair.
 template <int D>
 __global__ void __launch_bounds__(256)
-combine_tiles_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out,
+combine_tiles_kernel(const float* part_o, const float2* part_ml, __nv_bfloat16* __restrict__ out,
                      const int* __restrict__ segment_start, const int* __restrict__ first_pos, int num_segments, int n_q, int group,
                      int heads, int head0, int tokens_a_tile, int skip_single, int parts) {
   constexpr int V = D / 32;

@@ -69,8 +69,8 @@ __device__ __forceinline__ uint64_t mul_pairs(uint64_t a, uint64_t b) { uint64_t
 constexpr int STEP = 16;
 template <int STEPS>
 __global__ void __launch_bounds__(CHUNK_WARPS * 32, 9)
-beam_chunk_kernel(const float* __restrict__ logits, long long row_stride, int vocab, int beams, const float* __restrict__ scores,
-                  const int* __restrict__ ended, Best* __restrict__ best, Sum* __restrict__ sums) {
+beam_chunk_kernel(const float* logits, long long row_stride, int vocab, int beams, const float* scores,
+                  const int* ended, Best* best, Sum* sums) {
   __shared__ Best list[CHUNK_WARPS][WARP_LIST], kept[CHUNK_WARPS * MAX_BEAMS];
   __shared__ float warp_max_s[CHUNK_WARPS], warp_sum_s[CHUNK_WARPS];
   __shared__ unsigned short pair_s[CHUNK_WARPS][WARP_LIST];
@@ -226,9 +226,9 @@ beam_chunk_kernel(const float* __restrict__ logits, long long row_stride, int vo
 // One block per request.  HELD: offers a thread keeps in registers; beyond them they are read again.
 template <int MERGE_THREADS, int HELD>
 __global__ void __launch_bounds__(MERGE_THREADS)
-beam_merge_kernel(const Best* __restrict__ best, const Sum* __restrict__ sums, int chunks, int beams,
-                  const float* __restrict__ scores, const int* __restrict__ ended, int end_token, float* __restrict__ out_scores,
-                  int* __restrict__ out_tokens, int* __restrict__ out_parents, int* __restrict__ out_ended) {
+beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
+                  const float* scores, const int* ended, int end_token, float* out_scores,
+                  int* out_tokens, int* out_parents, int* out_ended) {
   constexpr int WARPS = MERGE_THREADS / 32, GROUP_LANES = MERGE_THREADS / GROUPS;
   __shared__ double lse[MAX_BEAMS], group_top[GROUPS], bound_s, list_v[LIST];
   __shared__ long long list_at[LIST];
@@ -389,8 +389,8 @@ struct Storages { Storage s[MAX_STORAGES]; int n; };
 
 template <typename V>
 __global__ void __launch_bounds__(256)
-beam_reorder_kernel(const int* __restrict__ parents, int beams, const int* __restrict__ tables, int table_stride, int width,
-                    const int* __restrict__ lengths, int page_size, int* __restrict__ new_tables, int new_stride,
+beam_reorder_kernel(const int* parents, int beams, const int* tables, int table_stride, int width,
+                    const int* lengths, int page_size, int* new_tables, int new_stride,
                     const __grid_constant__ Storages storages) {
   pdl_wait();
   const int row = blockIdx.x, request = row / beams, beam = row - request * beams, lane = threadIdx.x & 31;

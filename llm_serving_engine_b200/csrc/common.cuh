@@ -88,6 +88,8 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
 // all); what lies before pdl_wait() (setting up barriers, fetching weights) overlaps the
 // tail of the kernel before.  pdl_wait() returns when the earlier kernels have finished
 // and their writes are visible; it is a no-op when the launch carried no such permission.
+// What an earlier kernel wrote is not to be read through a `const T* __restrict__` parameter: the compiler takes such memory to be the
+// same during the whole launch and may move the load above pdl_wait() (it did: queries of the step before).
 inline int lse_pdl_enabled = 1;
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }

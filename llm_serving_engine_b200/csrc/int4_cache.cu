@@ -45,7 +45,7 @@ __device__ __forceinline__ __nv_bfloat16 bf16_of(double v) { return __float2bflo
 constexpr int THREADS = 256;
 template <typename TI, int D, int PAIRING, int TOKENS>
 __global__ void __launch_bounds__(THREADS, 4)
-rope_kv_write_int4_kernel(const TI* __restrict__ qkv, int n_partials, long long partial_stride, const float* __restrict__ bias,
+rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_stride, const float* __restrict__ bias,
                           const int* __restrict__ positions, const int* __restrict__ slot_mapping,
                           const float* __restrict__ inv_freq, __nv_bfloat16* __restrict__ q_out, unsigned char* __restrict__ k_codes,
                           __nv_bfloat162* __restrict__ k_scales, unsigned char* __restrict__ v_codes,
@@ -217,8 +217,8 @@ rope_kv_write_int4_kernel(const TI* __restrict__ qkv, int n_partials, long long 
 // Eight values a thread: keys (blockIdx.y = 0) or values (1) of the slots, as bfloat16.
 template <int D>
 __global__ void __launch_bounds__(256)
-kv_read_int4_kernel(const unsigned char* __restrict__ k_codes, const __nv_bfloat162* __restrict__ k_scales,
-                    const unsigned char* __restrict__ v_codes, const __nv_bfloat162* __restrict__ v_scales,
+kv_read_int4_kernel(const unsigned char* k_codes, const __nv_bfloat162* k_scales,
+                    const unsigned char* v_codes, const __nv_bfloat162* v_scales,
                     const int* __restrict__ slot_mapping, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                     int tokens, int n_kv, int page_size, long long num_slots) {
   constexpr int LANES = D / 8;

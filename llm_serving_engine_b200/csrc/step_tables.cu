@@ -13,10 +13,10 @@ namespace {
 constexpr int THREADS = 256;
 
 __global__ void __launch_bounds__(THREADS)
-step_tables_kernel(const int* __restrict__ first, const int* __restrict__ counts, const int* __restrict__ pages,
-                   const int* __restrict__ page_start, int requests, int page_size, int tokens, int row_blocks,
-                   int* __restrict__ segment_start, int* __restrict__ segment_of_token, int* __restrict__ positions,
-                   int* __restrict__ slots, int* __restrict__ contexts, int* __restrict__ tables, int table_stride, int width) {
+step_tables_kernel(const int* first, const int* counts, const int* pages,
+                   const int* page_start, int requests, int page_size, int tokens, int row_blocks,
+                   int* segment_start, int* segment_of_token, int* positions,
+                   int* slots, int* contexts, int* tables, int table_stride, int width) {
   __shared__ int ends[THREADS], warp_sums[THREADS / 32];
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

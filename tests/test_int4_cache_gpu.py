@@ -408,3 +408,38 @@ def test_portions_captured():
                 graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("splits", [1, 4, 24])
+def test_attention_behind_the_write_of_its_queries(splits):
+    """A graph of writes and attention that share a buffer for their queries, launches without a gap: each sees the write before it."""
+    g = torch.Generator().manual_seed(6)
+    layers, rows, n_q, n_kv, dim = 4, 3, 6, 2, 128
+    caches = [fill_cache(g, 24, n_kv, 16, dim) for _ in range(layers)]
+    tables = torch.arange(24).int().cuda().view(rows, 8)
+    segments, positions = torch.arange(rows).int().cuda(), torch.tensor([41, 100, 7]).int().cuda()
+    slots = (tables[segments.long(), positions.long() // 16] * 16 + positions % 16).int()
+    inv_freq = torch.full((dim // 2,), 0.01, device="cuda")
+    qkv = torch.empty((layers, rows, (n_q + 2 * n_kv) * dim), device="cuda")
+    q = torch.empty((rows, n_q, dim), dtype=torch.bfloat16, device="cuda")
+    outs = torch.empty((layers, rows, n_q, dim), dtype=torch.bfloat16, device="cuda")
+
+    def run(between):
+        for cache, x, out in zip(caches, qkv, outs):
+            ops.rope_kv_write_int4(x, None, positions, slots, inv_freq, q, *cache, n_q, n_kv, dim, 1)
+            between()
+            ops.paged_attention_decode_int4(q, *cache, out, tables, segments, positions, 0.09, num_splits=splits)
+            between()
+
+    run(torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(lambda: None)
+    for _ in range(4):
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        run(torch.cuda.synchronize)
+        want = outs.clone()
+        q.fill_(math.nan)
+        outs.zero_()
+        graph.replay()
+        assert torch.equal(outs, want)
