@@ -247,6 +247,9 @@ _SIGNATURES = {
     "lse_decode_layers": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p, c_void_p, c_float, c_void_p, c_int,
                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                           c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p],
+    "lse_attention_int4_tc_status": [],
+    "lse_attention_int4_tc_status_async": [c_void_p, c_void_p],
+    "lse_attention_int4_tc_status_reset": [],
     "lse_decode_layers_status": [],
     "lse_decode_layers_status_async": [c_void_p, c_void_p],
     "lse_decode_layers_status_reset": [],

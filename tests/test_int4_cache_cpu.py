@@ -113,3 +113,10 @@ def tables(**changes):
 def test_step_tables_refuse(changes, what):
     with pytest.raises(KernelError, match=what):
         tables(**changes)
+
+
+def test_status_words_are_read_by_declared_entry_points():
+    from llm_serving_engine_b200.kernels import library
+    for _, entry in ops._STATUS_WORDS:
+        for name in (entry, entry + "_async", entry + "_reset"):
+            assert name in library._SIGNATURES, name
