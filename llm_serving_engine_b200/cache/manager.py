@@ -25,7 +25,9 @@ Beyond it:
   itself stands behind the mixer's members.
 
 Storage layout of a group: [layer in group, 2 (keys, values), page, kv head,
-offset in page, head size]: the tokens of one page and one head are contiguous.
+offset in page, head size]: the tokens of one page and one head are contiguous.  With
+``CacheConfig.kv_bits`` 4 it holds codes, two a byte (uint8, half the head size), and
+``scale_storage`` a scale and a centre (bfloat16) for every row of a head.
 """
 from __future__ import annotations
 
@@ -37,7 +39,11 @@ import numpy as np
 import torch
 
 from ..config.runtime_config import CacheConfig
+from ..kernels import library
 from ..parts.base import PagedKV, PagedLatent, RequestState
+
+
+INT4_SOURCES = ("int4_cache", "attention_int4", "attention_int4_tcgen05")     # kernels of caches of 4 bits
 
 
 class CacheFullError(RuntimeError):
@@ -92,6 +98,7 @@ class CacheGroup:
     storage: torch.Tensor | None = None           # [len(layers), 2, pages, kv heads, page_size, head size], or
                                                   # [len(layers), 1, pages, page_size, width] for latent rows
     layer_slot: dict[int, int] = field(default_factory=dict)
+    scale_storage: torch.Tensor | None = None     # [len(layers), 2, pages, kv heads, page_size, 2] of codes of 4 bits
     value_storage: torch.Tensor | None = None     # [len(layers), pages, kv heads, page_size, value size] when values
                                                   # have a size of their own (storage then holds the keys alone)
 
@@ -112,6 +119,8 @@ class RequestCache:
     tables: list[list[int]] = field(default_factory=list)
     released: list[int] = field(default_factory=list)  # per group: logical pages given back so far
     tables_np: list = field(default_factory=list)      # per group: the same table as an int32 array (grown as needed)
+    lent: list[list[int]] = field(default_factory=list)     # per group: pages beside the table (the request's further beams')
+    lent_slots: list[int] = field(default_factory=list)
 
 
 @dataclass
@@ -124,6 +133,8 @@ class LayerCache:
     slot_mapping: torch.Tensor | None = None  # int32 [tokens]: page * page_size + offset of each row
     state: torch.Tensor | None = None         # [slots, *shape] of a mixer with fixed-size state
     group: int = -1
+    key_scales: torch.Tensor | None = None    # [pages, kv heads, page_size, 2]: keys and values are codes of 4 bits
+    value_scales: torch.Tensor | None = None
     parts: list | None = None                 # views of the members, for a mixer whose requirement is a tuple
 
 
@@ -163,6 +174,14 @@ class CacheManager:
                 single += [((layer, index), member) for index, member in enumerate(need)]
             else:
                 single.append((layer, need))
+        if config.kv_bits == 4:
+            if dtype != torch.bfloat16:
+                raise ValueError("a cache of 4 bits goes with bfloat16 models")
+            if any(isinstance(need, int) and not isinstance(need, bool) or isinstance(need, (PagedKV, PagedLatent)) and not getattr(need, "int4", False)
+                   for _, need in single):
+                raise ValueError("a layer of this model does not take a cache of 4 bits")
+            if self.device.type == "cuda":
+                library.require(INT4_SOURCES)
         for layer, need in single:
             if isinstance(need, (PagedKV, PagedLatent)):
                 group = by_need.get(need)
@@ -189,6 +208,10 @@ class CacheManager:
             elif group.need.value_dim in (0, group.need.head_dim):
                 shape = (len(group.layers), 2, config.num_blocks, group.need.num_kv_heads, self.page_size,
                          group.need.head_dim)
+                if config.kv_bits == 4:
+                    group.scale_storage = torch.zeros(shape[:5] + (2,), dtype=dtype, device=self.device)
+                    group.storage = torch.zeros(shape[:5] + (group.need.head_dim // 2,), dtype=torch.uint8, device=self.device)
+                    continue
             else:
                 shape = (len(group.layers), 1, config.num_blocks, group.need.num_kv_heads, self.page_size,
                          group.need.head_dim)
@@ -242,6 +265,20 @@ class CacheManager:
                 return False
         self._extend(request, after)
         return True
+
+    def lend(self, request_id: str, pages: int, slots: int) -> tuple[list[list[int]], list[int]]:
+        """``pages`` pages of every group and ``slots`` state slots beside the request's own, for beams that go on from its
+        cache; they go back with the request.  All or nothing."""
+        request = self.requests[request_id]
+        if any(pages > group.pool.free_pages for group in self.groups):
+            raise CacheFullError("paged KV cache has no free blocks")
+        if slots > len(self._free_slots):
+            raise CacheFullError("no free per-request state slot")
+        lent = [[group.pool.allocate(request_id) for _ in range(pages)] for group in self.groups]
+        taken = [self._free_slots.popleft() for _ in range(slots)]
+        request.lent = [had + new for had, new in zip(request.lent or [[] for _ in self.groups], lent)]
+        request.lent_slots += taken
+        return lent, taken
 
     def _extend(self, request: RequestCache, after: int) -> None:
         request_id = request.request_id
@@ -318,7 +355,11 @@ class CacheManager:
             for page in table:
                 if page >= 0:
                     group.pool.free(page, request_id)
+        for group, pages in zip(self.groups, request.lent):
+            for page in pages:
+                group.pool.free(page, request_id)
         self._free_slots.append(request.state_slot)
+        self._free_slots.extend(request.lent_slots)
 
     def free_all(self) -> None:
         for request_id in list(self.requests):
@@ -364,12 +405,16 @@ class CacheManager:
             view.values = storage[1] if storage.shape[0] > 1 else None
             if group.value_storage is not None:
                 view.values = group.value_storage[group.layer_slot[source]]
+            if group.scale_storage is not None:
+                view.key_scales, view.value_scales = group.scale_storage[group.layer_slot[source]]
         if source in self.states.tensors:
             view.state = self.states.tensors[source]
         return view
 
     # -- statistics ------------------------------------------------------------
     def bytes_per_page(self, group: CacheGroup) -> int:
+        if group.scale_storage is not None:      # half a byte a number, four bytes a row
+            return len(group.layers) * self.page_size * group.need.num_kv_heads * 2 * (group.need.head_dim // 2 + 4)
         per_token = (group.need.width if isinstance(group.need, PagedLatent)
                      else group.need.num_kv_heads * (group.need.head_dim + (group.need.value_dim or group.need.head_dim)))
         return len(group.layers) * self.page_size * per_token * torch.empty((), dtype=self.dtype).element_size()

@@ -176,7 +176,7 @@ class _Runtime:
 
         args = self.args
         return LLMEngine(self.model, self.tokenizer,
-                         cache_config=CacheConfig(block_size=args.block_size, num_blocks=args.num_blocks),
+                         cache_config=CacheConfig(block_size=args.block_size, num_blocks=args.num_blocks, kv_bits=args.kv_bits),
                          scheduler_config=SchedulerConfig(max_batch_size=batch_size or args.batch_size,
                                                           max_tokens_per_step=args.max_tokens_per_step, policy=policy),
                          scheduler_mode=mode, prefill_chunk_size=args.prefill_chunk_size,
@@ -295,6 +295,7 @@ def _engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--batch-size", type=int, default=16)
     parser.add_argument("--block-size", type=int, default=16)
     parser.add_argument("--num-blocks", type=int, default=1024)
+    parser.add_argument("--kv-bits", type=int, choices=(0, 4), default=0, help="bits of a cached key's or value's number (0: the model's type)")
     parser.add_argument("--prefill-chunk-size", type=int, default=2048)
     parser.add_argument("--max-tokens-per-step", type=int, default=2048)
     parser.add_argument("--seed", type=int, default=7)

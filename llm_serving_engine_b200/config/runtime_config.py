@@ -9,13 +9,17 @@ from dataclasses import dataclass
 class CacheConfig:
     """``block_size`` tokens per page, ``num_blocks`` pages in every layer group's pool;
     ``num_state_slots`` fixed-size per-request state slots (0 = as many as the
-    scheduler's ``max_batch_size``)."""
+    scheduler's ``max_batch_size``).  ``kv_bits``: bits of a cached key's or value's number, 0 for the model's
+    type, 4 for codes with a scale and a centre a row (bfloat16 models whose attentions take them)."""
 
     block_size: int = 16
     num_blocks: int = 1_024
     num_state_slots: int = 0
+    kv_bits: int = 0
 
     def __post_init__(self) -> None:
+        if self.kv_bits not in (0, 4):
+            raise ValueError("kv_bits must be 0 (the model's type) or 4")
         if self.block_size <= 0 or self.num_blocks <= 0 or self.num_state_slots < 0:
             raise ValueError("block_size and num_blocks must be positive")
 

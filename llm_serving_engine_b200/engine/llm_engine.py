@@ -21,6 +21,7 @@ from ..cache.manager import CacheFullError, CacheManager
 from ..config.runtime_config import CacheConfig, SchedulerConfig
 from ..models import cache_requirements
 from ..sampling.sampler import GenerationConfig, Sampler
+from .beam_search import BeamSearch
 from .scheduler import GenerationRequest, Scheduler
 from .step import StepEntry, StepRunner
 
@@ -179,6 +180,21 @@ class LLMEngine:
             if state.request_id in errors:
                 raise errors[state.request_id]
         return [state.output for state in states]
+
+    def beam_search(self, prompts, beams: int, max_new_tokens: int, end_token: int) -> list:
+        """The best ``beams`` continuations of every prompt (token ids or text), the best first: lists of
+        ``engine.Beam``.  Synchronous, and only while no request is being generated."""
+        if self._closed:
+            raise RuntimeError("engine is closed")
+        if not self.scheduler.idle or self.cache.requests:
+            raise RuntimeError("beam search runs while no request is being generated")
+        if self.tokenizer is None and any(isinstance(prompt, str) for prompt in prompts):
+            raise ValueError("a text prompt needs a tokenizer")
+        tokens = [self.tokenizer.encode(prompt) if isinstance(prompt, str) else [int(token) for token in prompt] for prompt in prompts]
+        vocab = self.model.vocab_size
+        if any(prompt and (min(prompt) < 0 or max(prompt) >= vocab) for prompt in tokens):
+            raise ValueError(f"prompt holds a token id outside [0, {vocab})")
+        return BeamSearch(self.runner, beams, end_token).search(tokens, max_new_tokens)
 
     # -- the loop ------------------------------------------------------------------
     async def _run(self) -> None:

@@ -30,6 +30,7 @@ import torch
 
 from ..cache.manager import CacheFullError, CacheManager, LayerCache
 from ..kernels import ops
+from ..parts.attention import int4_launch_class
 
 
 @dataclass
@@ -328,8 +329,13 @@ class StepRunner:
         step.want_rows = dev[lay.want[0]:lay.want[1]]
         group_maps = [dev[lo:hi] for lo, hi in lay.maps]
         group_tables = [dev[lo:hi].view(lay.segments, lay.table_width) for lo, hi in lay.tables]
+        return step, self.layer_caches(group_maps, group_tables)
+
+    def layer_caches(self, group_maps: list, group_tables: list) -> list[LayerCache]:
+        """What every layer run's mixer sees in a step with these cache slots and block tables (one of each per group)."""
         def bind(view: LayerCache) -> LayerCache:
-            layer_cache = LayerCache(keys=view.keys, values=view.values, state=view.state, group=view.group)
+            layer_cache = LayerCache(keys=view.keys, values=view.values, state=view.state, group=view.group,
+                                     key_scales=view.key_scales, value_scales=view.value_scales)
             if view.group >= 0:
                 layer_cache.slot_mapping = group_maps[view.group]
                 layer_cache.block_tables = group_tables[view.group]
@@ -337,7 +343,7 @@ class StepRunner:
                 layer_cache.parts = [bind(part) for part in view.parts]
             return layer_cache
 
-        return step, [bind(view) for view in self._layer_views]
+        return [bind(view) for view in self._layer_views]
 
     def prepare(self, entries: list[StepEntry], validated: bool = False):
         """Reserve, pack and upload a step; returns ``(StepContext, [LayerCache per layer run])``."""
@@ -427,6 +433,8 @@ class StepRunner:
         counts = [len(entry.tokens) for entry in entries]
         contexts = [self.cache.requests[entry.request_id].length + count for entry, count in zip(entries, counts)]
         signature = self.model.launch_signature(counts, contexts) if hasattr(self.model, "launch_signature") else ()
+        if self.cache.config.kv_bits == 4:
+            signature = (*signature, int4_launch_class(counts, contexts))
         key = ("portions", tokens, segments, places, self._graph_width(self._pages_after(entries)), signature)
         slot = self._portion_graphs.get(key)
         if slot is None:

@@ -39,6 +39,16 @@ ROWS_KERNEL_BLOCKS = 256
 # of 128, 640 chunks, 16.6 against 19.7; at 1,024 chunks the two are alike, 64 rows behind 2,000 keys are slower).
 GENERIC_ROWS_UP_TO, GENERIC_ROWS_CHUNKS = 64, 640
 
+INT4_SHORT_CONTEXT = 8192     # keys that a captured decode step holds at most unless it counts as one over long contexts
+
+
+def int4_launch_class(counts: list[int], contexts: list[int]) -> tuple[int, int, bool]:
+    """What the launches over 4-bit pages of a step with prompt portions depend on: upper bounds (powers of two) on the keys of all
+    requests and of one, and whether single tokens go to the kernel for rows."""
+    def bound(keys: int) -> int:
+        return 1 << max(10, (keys - 1).bit_length())
+    return bound(sum(contexts)), bound(max(contexts)), max(counts) > 1 and any(count == 1 for count in counts)
+
 
 @register_mixer("gqa_attention")
 class GroupedQueryAttention(Mixer):
@@ -91,7 +101,9 @@ class GroupedQueryAttention(Mixer):
 
     @classmethod
     def cache_requirement(cls, params, hidden_size):
-        return PagedKV(int(params["num_kv_heads"]), int(params["head_dim"]), int(params.get("window", 0)))
+        window, position = int(params.get("window", 0)), POSITION_ENCODINGS.get(params["position"]["kind"])
+        return PagedKV(int(params["num_kv_heads"]), int(params["head_dim"]), window,
+                       int4=window == 0 and int(params["head_dim"]) in (64, 128) and position.int4)
 
     def prompt_kernel(self, segment_counts: list[int], page_size: int | None = None) -> str:
         """"tcgen05" or "mma": the kernel a step with prompt portions takes (the rule at the top of this file)."""
@@ -175,6 +187,22 @@ class GroupedQueryAttention(Mixer):
         ops.paged_attention_generic(*arguments, segment_start=step.segment_start, segment_first_position=step.segment_first_position,
                                     skip_single=singles, max_context=longest)
 
+    def _int4_attention(self, q, cache, attended, step):
+        """Over pages that hold keys and values in 4 bits: single tokens row by row, portions on the tensor cores."""
+        pages = (cache.keys, cache.key_scales, cache.values, cache.value_scales)
+        if step.decode_only:      # a captured step's contexts grow until its tables are full, or reach what counts as long
+            longest = step.max_context or (0 if step.long_context else INT4_SHORT_CONTEXT)
+            ops.paged_attention_decode_int4(q, *pages, attended, cache.block_tables, step.segment_of_token, step.positions, self.scale,
+                                            max_context=longest)
+            return
+        counts = [segment.count for segment in step.segments]
+        keys, longest, singles = int4_launch_class(counts, [segment.first_position + segment.count for segment in step.segments])
+        if singles:
+            ops.paged_attention_decode_int4(q, *pages, attended, cache.block_tables, step.segment_of_token, step.positions, self.scale,
+                                            max_context=longest, segment_start=step.segment_start)
+        ops.paged_attention_prefill_int4(q, *pages, attended, cache.block_tables, step.segment_start, step.segment_first_position, self.scale,
+                                         keys=keys, skip_single=singles)
+
     def forward(self, x, step, cache):
         tokens = x.shape[0]
         # bias is added with the rotation, in float32; at most 8 partial sums: the rotary kernel fetches them in one go
@@ -182,7 +210,9 @@ class GroupedQueryAttention(Mixer):
         q = torch.empty((tokens, self.n_q, self.head_dim), dtype=x.dtype, device=x.device)
         self.position.encode_and_store(qkv, self.qkv_bias, step, cache, q, self.n_q, self.n_kv, self.head_dim)
         attended = torch.empty_like(q)
-        if ops.attention_mma_supported(self.head_dim, self.n_q, self.n_kv, x.dtype, self.window):
+        if cache.key_scales is not None:
+            self._int4_attention(q, cache, attended, step)
+        elif ops.attention_mma_supported(self.head_dim, self.n_q, self.n_kv, x.dtype, self.window):
             if step.decode_only:
                 splits = ops.decode_splits(tokens, self.n_q, self.n_kv, step.max_context, getattr(step, "long_context", False),
                                            getattr(step, "many_keys", False))

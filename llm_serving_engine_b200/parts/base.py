@@ -49,13 +49,15 @@ class PagedKV:
     """The mixer keeps keys and values of every token in pages.  ``window`` > 0:
     only the last ``window`` keys are read, older pages are given back.
     ``value_dim`` > 0: a value has this size instead of ``head_dim`` (keys and values then lie in two tensors).
-    ``keep_first`` > 0 (with a window): the request's first so many keys are read for ever, their pages stay."""
+    ``keep_first`` > 0 (with a window): the request's first so many keys are read for ever, their pages stay.
+    ``int4``: the mixer also takes pages that hold keys and values in 4 bits (``CacheConfig.kv_bits``)."""
 
     num_kv_heads: int
     head_dim: int
     window: int = 0
     value_dim: int = 0
     keep_first: int = 0
+    int4: bool = field(default=False, compare=False)
 
 
 @dataclass(frozen=True)
@@ -153,6 +155,8 @@ class Norm(Part):
 
 
 class PositionEncoding(Part):
+    int4 = False           # whether encode_and_store also writes pages of 4 bits (cache.key_scales is not None)
+
     def encode_and_store(self, qkv, bias, step, cache, q_out, n_q, n_kv, head_dim) -> None:
         raise NotImplementedError
 
