@@ -9,8 +9,8 @@
 // Storage: codes uint8 [page][kv head][offset][D / 2], byte b holding d = 2 b in its low and 2 b + 1 in its high half; scales
 // bfloat16 [page][kv head][offset][2] = (s, c).
 //
-// Everything up to the code is worked out in 64 bits: a code next to the border between two flips with the last bit of x, and a
-// flipped code is a whole step of the row's range.  With float32 rotations about two codes in a million depended on how the
+// The code is that of 64-bit arithmetic throughout: a code next to the border between two flips with the last bit of x, and a
+// flipped code is a whole step of the row's range.  (Scale and centre come from float32 where that provably gives the same.)  With float32 rotations about two codes in a million depended on how the
 // sine was rounded.  (FP64 runs at half the float32 rate here; sines are taken once a token, not once a head.)
 #include "common.cuh"
 
@@ -36,12 +36,14 @@ __device__ __forceinline__ double shfl_xor_double(double v, int o) {
 // double to bfloat16 by way of float32, as a tensor library converts
 __device__ __forceinline__ __nv_bfloat16 bf16_of(double v) { return __float2bfloat16_rn((float)v); }
 
-// One block = TOKENS tokens x their query heads (blockIdx.y < q_blocks), or x their key and value heads.  It works out the tokens' sines
-// (a thread each), then its threads walk (token, head) rows with the next row's projections on their way.  A thread owns eight
-// values of a head: pairing 0 the neighbours 8 c .. 8 c + 7 (four pairs), pairing 1 the runs 4 c .. and D / 2 + 4 c .. (pairs across
+// One block = TOKENS tokens x their key and value heads (blockIdx.y < kv_blocks), or x their query heads.  It works out the tokens' sines
+// (a thread each), then its threads walk the heads of a token each, with the next head's projections on their way.  A thread owns
+// eight values of a head: pairing 0 the neighbours 8 c .. 8 c + 7 (four pairs), pairing 1 the runs 4 c .. and D / 2 + 4 c .. (pairs across
 // the halves).  LANES = D / 8 threads share a head and find its extremes by shuffles.
-// What bounds it: the instructions of the 64-bit part.  2,001 rows of 40 / 8 heads of 128 in float32 (90 MB) take 27 us, 41 with a block
-// that walked all heads of a token in 64 bits, one pass after the other.
+// What bounds it: neither memory nor instructions alone (2,001 rows of 40 / 8 heads of 128 in float32: 82 MB in 27.4 us, 3.0 TB/s; 52% of
+// the issue slots), but a block's chain of loads, sines, 64-bit rotations and shuffles.  The keys' and values' blocks alone take 16.3 us,
+// the queries' alone 18.0; either without the sines 0.1 less.  Extremes, scale and centre all in 64 bits: 32.3 us.  Two rows on
+// their way instead of one: 29.3; two, four or eight tokens a block, blocks of 128 threads, either kind of block first: 27.0 to 28.2.
 constexpr int THREADS = 256;
 template <typename TI, int D, int PAIRING, int TOKENS>
 __global__ void __launch_bounds__(THREADS, 4)
@@ -55,10 +57,14 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
   __shared__ double2 turn_s[TOKENS * HALF];      // cosines and sines of the tokens' angles
   pdl_launch_dependents();
   const int t0 = blockIdx.x * TOKENS, count = min(TOKENS, tokens - t0);
-  const bool queries = (int)blockIdx.y < q_blocks;
+  const int kv_blocks = (int)gridDim.y - q_blocks;      // first in the grid: they take longer
+  const bool queries = (int)blockIdx.y >= kv_blocks;
   const int heads = queries ? n_q : 2 * n_kv, head0 = queries ? 0 : n_q;         // of a token; its first among a row's heads
-  const int step = HEADS * (queries ? q_blocks : (int)gridDim.y - q_blocks), rows = count * heads;
-  const int begin = (queries ? (int)blockIdx.y : (int)blockIdx.y - q_blocks) * HEADS;
+  // a thread keeps its token and goes on by `step` heads
+  constexpr int AT_ONCE = HEADS / TOKENS;
+  const int step = AT_ONCE * (queries ? q_blocks : kv_blocks), begin = (queries ? (int)blockIdx.y - kv_blocks : (int)blockIdx.y) * AT_ONCE;
+  const int token = threadIdx.x / LANES % TOKENS, offset = threadIdx.x / LANES / TOKENS;
+  const bool here = token < count;
   const int c = threadIdx.x % LANES;
   const int e0 = PAIRING == 0 ? 8 * c : 4 * c, e1 = PAIRING == 0 ? 8 * c + 4 : HALF + 4 * c;
   // positions, slots, frequencies and bias are the step's or the model's own data: read before the wait for the kernel that makes the
@@ -84,12 +90,12 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
 #pragma unroll
     for (int j = 0; j < 4; ++j) { to[j] = lo[j]; to[4 + j] = hi[j]; }
   };
-  struct Place { int row, token, head; };      // of this thread's row; head counted from head0
-  auto load_row = [&](const Place& p, float (&to)[8]) {
+  const TI* const mine_in = qkv + (size_t)(t0 + token) * qkv_stride + (size_t)head0 * D;      // (read only where the token is there)
+  auto load_row = [&](int head, float (&to)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) to[j] = 0.f;
-    if (p.row >= rows) return;
-    const TI* row = qkv + (size_t)(t0 + p.token) * qkv_stride + (size_t)(head0 + p.head) * D;
+    if (!here || head >= heads) return;
+    const TI* row = mine_in + head * D;
     if (n_partials == 1) {
       load_eight(row, to);
       return;
@@ -102,29 +108,34 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
       for (int j = 0; j < 8; ++j) to[j] += a[j];
     }
   };
-  auto at_row = [&](int row) { Place p; p.row = row; p.token = (unsigned)row / (unsigned)heads; p.head = row - p.token * heads; return p; };
-  Place now = at_row(begin + threadIdx.x / LANES);
   float g[8];
-  load_row(now, g);
+  load_row(begin + offset, g);
   __syncthreads();
-  for (int base = begin; base < rows; base += step) {      // the same in the whole block: shuffles take whole warps
-    const Place next = at_row(now.row + step);
+  float2 turn_q[4];
+  if (queries) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) turn_q[j] = reinterpret_cast<const float2*>(turn_s)[token * HALF + 4 * c + j];
+  }
+  const int slot = !queries && here ? LSE_CHECKED(slot_mapping[t0 + token], -1, (int)num_slots, -1, LSE_CHECK_CACHE_SLOT) : -1;
+  const size_t page = (unsigned)max(slot, 0) / (unsigned)page_size, off = (unsigned)max(slot, 0) % (unsigned)page_size;
+  for (int base = begin; base < heads; base += step) {      // the same in the whole block: shuffles take whole warps
+    const int head = base + offset;
+    const bool live = here && head < heads;
     float ahead[8];
-    load_row(next, ahead);
+    load_row(head + step, ahead);
     float b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) b[j] = 0.f;
-    if (now.row < rows && bias) load_eight(bias + (size_t)(head0 + now.head) * D, b);
+    if (live && bias) load_eight(bias + (size_t)(head0 + head) * D, b);
     if (queries) {
-      if (now.row < rows) {
-        const float2* turn = reinterpret_cast<const float2*>(turn_s) + now.token * HALF + 4 * c;
+      if (live) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] += b[j];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float& x = PAIRING == 0 ? g[2 * j] : g[j];
           float& y = PAIRING == 0 ? g[2 * j + 1] : g[4 + j];
-          const float rx = x * turn[j].x - y * turn[j].y, ry = y * turn[j].x + x * turn[j].y;
+          const float rx = x * turn_q[j].x - y * turn_q[j].y, ry = y * turn_q[j].x + x * turn_q[j].y;
           x = rx; y = ry;
         }
         uint32_t w[4];
@@ -133,7 +144,7 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
           const __nv_bfloat162 v = __floats2bfloat162_rn(g[2 * j], g[2 * j + 1]);
           w[j] = *reinterpret_cast<const uint32_t*>(&v);
         }
-        __nv_bfloat16* dst = q_out + ((size_t)t0 * n_q + now.row) * D;
+        __nv_bfloat16* dst = q_out + ((size_t)(t0 + token) * n_q + head) * D;
         if (PAIRING == 0) {
           *reinterpret_cast<uint4*>(dst + e0) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
@@ -142,8 +153,7 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
         }
       }
     } else {
-      const bool is_k = now.head < n_kv;
-      const int slot = now.row < rows ? LSE_CHECKED(slot_mapping[t0 + now.token], -1, (int)num_slots, -1, LSE_CHECK_CACHE_SLOT) : -1;
+      const bool is_k = head < n_kv;
       double x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (double)g[j];
@@ -151,53 +161,91 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += (double)b[j];
       }
-      if (is_k && now.row < rows) {
+      if (is_k && live) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const double2 turn = turn_s[now.token * HALF + 4 * c + j];
+          const double2 turn = turn_s[token * HALF + 4 * c + j];
           double& p = PAIRING == 0 ? x[2 * j] : x[j];
           double& q = PAIRING == 0 ? x[2 * j + 1] : x[4 + j];
           const double rp = p * turn.x - q * turn.y, rq = q * turn.x + p * turn.y;
           p = rp; q = rq;
         }
       }
-      double low = x[0], high = x[0], all = x[0] * 0.0;      // `all`: zero where every value is finite
-#pragma unroll
-      for (int j = 1; j < 8; ++j) {
-        low = x[j] < low ? x[j] : low;
-        high = x[j] > high ? x[j] : high;
-        all = fma(x[j], 0.0, all);
-      }
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) {
-        const double l = shfl_xor_double(low, o), h = shfl_xor_double(high, o);
-        low = l < low ? l : low;
-        high = h > high ? h : high;
-      }
       // a row's lanes are LANES neighbours of a warp
       const unsigned mine = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
-      const bool whole = (__ballot_sync(0xffffffffu, all == 0.0) & mine) == mine;
-      if (slot >= 0) {
-        __nv_bfloat16 scale = bf16_of((high - low) / 15.0);
-        __nv_bfloat16 centre = bf16_of(low + 8.0 * (double)__bfloat162float(scale));
-        if (!whole) { scale = __float2bfloat16_rn(0.f); centre = __float2bfloat16_rn(__int_as_float(0x7fc00000)); }
-        const double s = (double)__bfloat162float(scale), m = (double)__bfloat162float(centre);
-        const double inverse = s != 0.0 ? 1.0 / s : 0.0;
-        uint32_t code[2] = {0u, 0u};      // four codes each: those of e0 .., those of e1 ..
+      __nv_bfloat16 scale, centre;
+      bool whole = true;       // every value of the row is finite
+      {
+        // The extremes as float32: scale and centre are those of the exact ones where either end of what these can be off by
+        // (and more: half a unit of the last place each, then two roundings of each expression) rounds to the same bfloat16.
+        float low = (float)x[0], high = low, none = low * 0.f;      // `none`: zero where every value is finite
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+          const float v = (float)x[j];
+          low = fminf(low, v); high = fmaxf(high, v);
+          none = fmaf(v, 0.f, none);
+        }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) {
+          low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+          high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        }
+        const float range = high - low, floor = range != 0.f ? 0x1p-120f : 0.f, off = fmaf(0x1p-21f, fabsf(high) + fabsf(low), floor);
+        const float s0 = __bfloat162float(__float2bfloat16_rn((range - off) * (1.f / 15.f)));
+        scale = __float2bfloat16_rn((range + off) * (1.f / 15.f));
+        const float s1 = __bfloat162float(scale), at = fmaf(8.f, s1, low), at_off = fmaf(0x1p-21f, fabsf(low) + 8.f * s1, floor);
+        const float c0 = __bfloat162float(__float2bfloat16_rn(at - at_off));
+        centre = __float2bfloat16_rn(at + at_off);
+        if (!__all_sync(0xffffffffu, none == 0.f && range < 1e37f && s0 == s1 && c0 == __bfloat162float(centre))) {
+          double lo = x[0], hi = x[0], all = x[0] * 0.0;
+#pragma unroll 1
+          for (int o = 0; o < LANES; o = o == 0 ? 1 : o << 1) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
+              if (o > 0) break;
+              lo = x[j] < lo ? x[j] : lo;
+              hi = x[j] > hi ? x[j] : hi;
+              all = fma(x[j], 0.0, all);
+            }
+            const double l = shfl_xor_double(lo, o), h = shfl_xor_double(hi, o);
+            lo = l < lo ? l : lo;
+            hi = h > hi ? h : hi;
+          }
+          whole = (__ballot_sync(0xffffffffu, all == 0.0) & mine) == mine;
+          scale = bf16_of((hi - lo) / 15.0);
+          centre = bf16_of(lo + 8.0 * (double)__bfloat162float(scale));
+          if (!whole) { scale = __float2bfloat16_rn(0.f); centre = __float2bfloat16_rn(__int_as_float(0x7fc00000)); }
+        }
+      }
+      if (live && slot >= 0) {
+        const float s_float = __bfloat162float(scale);
+        const double s = (double)s_float, m = (double)__bfloat162float(centre), half = 0.5 * s;
+        double inverse = (double)__fdividef(1.f, s_float);      // (an estimate will do)
+        if (!(s_float >= 0x1p-120f && s_float <= 0x1p120f)) inverse = s != 0.0 ? 1.0 / s : 0.0;
+        // the quotient (x - c) / s to nearest, halves to even: its estimate, rounded by the addition of a number whose last place is 1,
+        // is off by one at most, and what is left of x decides (exactly: rows that come in bfloat16 do lie half way between two codes)
+        constexpr double ONES = 0x1.8p52;
+        int q[8];
+        bool near = false;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          // the quotient (x - c) / s to nearest, halves to even: its estimate is off by one at most, and what is left of x decides
-          // (exactly: rows that come in bfloat16 do lie half way between two codes)
-          const double from_centre = x[j] - m;
-          int q = whole ? __double2int_rn(from_centre * inverse) : 0;
-          const double twice = 2.0 * fma(-(double)q, s, from_centre);
-          if (twice > s || (twice == s && (q & 1))) ++q;
-          else if (twice < -s || (twice == -s && (q & 1))) --q;
-          if (!whole || s == 0.0) q = 0;
-          code[j >> 2] |= (uint32_t)(min(max(q, -8), 7) + 8) << (4 * (j & 3));
+          const double from_centre = x[j] - m, rounded = fma(from_centre, inverse, ONES);
+          q[j] = __double2loint(rounded);
+          near |= fabs(fma(ONES - rounded, s, from_centre)) >= half;
         }
-        const size_t page = (unsigned)slot / (unsigned)page_size, off = (unsigned)slot % (unsigned)page_size;
-        const size_t place = (page * n_kv + (is_k ? now.head : now.head - n_kv)) * page_size + off;
+        if (near) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const double from_centre = x[j] - m, twice = 2.0 * fma(-(double)q[j], s, from_centre);
+            if (twice > s || (twice == s && (q[j] & 1))) ++q[j];
+            else if (twice < -s || (twice == -s && (q[j] & 1))) --q[j];
+          }
+        }
+        uint32_t code[2] = {0u, 0u};      // four codes each: those of e0 .., those of e1 ..
+#pragma unroll
+        for (int j = 0; j < 8; ++j) code[j >> 2] |= (uint32_t)(min(max(q[j], -8), 7) + 8) << (4 * (j & 3));
+        if (!whole || s == 0.0) code[0] = code[1] = 0x8888u;
+        const size_t place = (page * n_kv + (is_k ? head : head - n_kv)) * page_size + off;
         unsigned char* dst = (is_k ? k_codes : v_codes) + place * (D / 2);
         if (PAIRING == 0) {
           *reinterpret_cast<uint32_t*>(dst + 4 * c) = code[0] | code[1] << 16;
@@ -208,7 +256,6 @@ rope_kv_write_int4_kernel(const TI* qkv, int n_partials, long long partial_strid
         if (c == 0) (is_k ? k_scales : v_scales)[place] = __nv_bfloat162(scale, centre);
       }
     }
-    now = next;
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] = ahead[j];
   }

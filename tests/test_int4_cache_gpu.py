@@ -443,3 +443,27 @@ def test_attention_behind_the_write_of_its_queries(splits):
         outs.zero_()
         graph.replay()
         assert torch.equal(outs, want)
+
+
+@pytest.mark.parametrize("dim,pairing", [(64, 0), (128, 1)])
+def test_write_of_rows_on_the_borders_of_rounding(dim, pairing):
+    """Ranges and centres half way between two bfloat16 numbers, or a last place of float32 beside, and values half way between codes."""
+    g = torch.Generator().manual_seed(dim)
+    tokens, n_q, n_kv = 400, 1, 4
+    x = torch.randint(-128, 128, (tokens, n_q + 2 * n_kv, dim), generator=g).float() / 16
+    lows = torch.randint(-64, 0, (tokens, n_q + 2 * n_kv), generator=g).float() / 8
+    steps = (torch.randint(256, 512, lows.shape, generator=g).float() + 0.5) / 512           # half way between two of 8 bits
+    x = torch.maximum(torch.minimum(x, (lows + 15 * steps)[..., None]), lows[..., None])
+    x[..., 5], x[..., dim - 3] = lows, lows + 15 * steps
+    beside = torch.randint(-1, 2, lows.shape, generator=g)
+    x[..., 5] = torch.where(beside == 0, x[..., 5], torch.nextafter(x[..., 5], beside.float() * 1e9))
+    slots = torch.arange(tokens).int().cuda()
+    cache = empty_cache(tokens // 16, n_kv, 16, dim)
+    q = torch.empty((tokens, n_q, dim), dtype=torch.bfloat16, device="cuda")
+    zero = torch.zeros(dim // 2, device="cuda")               # no angles: a rotation that changes nothing
+    ops.rope_kv_write_int4(x.flatten(1).cuda(), None, slots, slots, zero, q, *cache, n_q, n_kv, dim, pairing)
+    page, at = slots.long() // 16, slots.long() % 16
+    for rows, codes, scales in ((x[:, n_q:n_q + n_kv], cache[0], cache[1]), (x[:, n_q + n_kv:], cache[2], cache[3])):
+        u, s, c = plain.quantise(rows.to(D64).cuda())
+        assert torch.equal(scales[page, :, at], torch.stack([s, c], -1).bfloat16())
+        assert torch.equal(codes[page, :, at], plain.pack(u))
