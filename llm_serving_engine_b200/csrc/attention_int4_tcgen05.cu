@@ -42,7 +42,7 @@ constexpr float KEY_SCALE = 1.0f / 256.0f, QUERY_SCALE = 1.0f / 16.0f, SCORE_SCA
 
 __device__ int lse_attn_int4_tc_error;
 
-enum Bar { B_Q = 0, B_KF = 1, B_KE = 3, B_VF = 5, B_VE = 7, B_SF = 9, B_PF = 11, B_SR = 13, B_OD = 15, B_QC = 17, B_COUNT = 18 };
+enum Bar { B_Q = 0, B_KF = 1, B_KE = 3, B_VF = 5, B_VE = 7, B_SF = 9, B_PF = 11, B_SR = 13, B_OD = 15, B_COUNT = 17 };
 
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x, 2^-inf = 0
   float y;
@@ -62,33 +62,85 @@ __device__ __forceinline__ uint32_t instr_desc_f16(int m, int n, bool a_mn, bool
 }
 template <int D> constexpr size_t attend_smem() { return 1024 + (size_t)(D / 64) * HALF_BYTES * (1 + 2 * GROUPS) + (size_t)GROUPS * 2 * HALF_BYTES + 256; }
 
-// Key tiles of the requests before `seg`, by a whole warp: request s holds the keys 0 .. its last row's position.
-__device__ __forceinline__ int tiles_before(const int* __restrict__ segment_start, const int* __restrict__ first_pos, int seg) {
-  int sum = 0;
-  for (int s = threadIdx.x & 31; s < seg; s += 32) {
-    const int rows = segment_start[s + 1] - segment_start[s];
-    sum += rows > 0 ? max(0, first_pos[s] + rows + BN - 1) / BN : 0;
-  }
+// What a block works on: the rank-th tile of rows, counted from the last request's last one backwards (late tiles walk the most keys and
+// start first; ranks beyond the number of tiles have none: seg = -1).  The first warp looks at 32 requests at a time, once where there
+// are no more, and leaves everything in `work`; the block has to meet before it is read.
+struct Work { int seg, r0, rows, first_row, first_pos, tile0; };
+__device__ __forceinline__ void find_work(const int* segment_start, const int* first_pos, int num_segments, int tokens_a_tile, int skip_single,
+                                          int rank, Work* work) {
+  const int lane = threadIdx.x & 31;
+  struct Request { int start, rows, first, tiles, key_tiles; };
+  auto look = [&](int s) {
+    Request r = {0, 0, 0, 0, 0};
+    if (s < num_segments) {
+      r.start = segment_start[s];
+      r.rows = max(segment_start[s + 1] - r.start, 0);
+      r.first = first_pos[s];
+      r.tiles = r.rows == 1 && skip_single ? 0 : (r.rows + tokens_a_tile - 1) / tokens_a_tile;
+      r.key_tiles = r.rows > 0 ? (max(0, r.first + r.rows) + BN - 1) / BN : 0;
+    }
+    return r;
+  };
+  const Request first = look(lane);
+  int all = first.tiles;
+  for (int base = 32; base < num_segments; base += 32) all += look(base + lane).tiles;
+  const int wanted = __reduce_add_sync(0xffffffffu, all) - 1 - rank;
+  if (lane == 0) work->seg = -1;
+  __syncwarp();
+  int before = 0, keys_before = 0;
+  for (int base = 0; base < num_segments && wanted >= before; base += 32) {
+    const Request r = base == 0 ? first : look(base + lane);
+    int incl = r.tiles, keys_incl = r.key_tiles;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o), k = __shfl_up_sync(0xffffffffu, keys_incl, o);
+      if (lane >= o) { incl += v; keys_incl += k; }
+    }
+    const int at = wanted - before - (incl - r.tiles);
+    if (at >= 0 && at < r.tiles) *work = {base + lane, at * tokens_a_tile, r.rows, r.start, r.first, keys_before + keys_incl - r.key_tiles};
+    before += __shfl_sync(0xffffffffu, incl, 31);
+    keys_before += __shfl_sync(0xffffffffu, keys_incl, 31);
+  }
 }
 
 // ------------------------------------------------------------------ expand
 // One block = EXPAND_KEYS keys of a tile and one head, keys and values; 256 threads, LANES = D / 8 of them a row, eight values each, all loads
 // of a thread on their way together (a block a tile, eight rows a thread one after the other: 17 us for 51 tiles of two heads).
 constexpr int EXPAND_KEYS = 32;
+constexpr int QUERY_PIECES = 4;      // 16 bytes each, of a thread of the blocks behind those (blockIdx.z), which make the queries float16
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_int4_kernel(const unsigned char* k_codes, const __nv_bfloat162* k_scales,
                    const unsigned char* v_codes, const __nv_bfloat162* v_scales, uint4* __restrict__ k_out,
                    uint4* __restrict__ v_out, const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
                    const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size, int num_pages, int capacity,
-                   int skip_single) {
+                   int skip_single, const uint4* q, uint4* q_out, long long q_pieces) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES, MINE = EXPAND_KEYS / ROWS;      // rows at once, rows of a thread
   __shared__ int found[3];
   pdl_launch_dependents();
   const int tile = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  if (blockIdx.z >= BN / EXPAND_KEYS) {      // queries
+    pdl_wait();
+    const long long block = ((long long)(blockIdx.z - BN / EXPAND_KEYS) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    uint4 w[QUERY_PIECES];
+#pragma unroll
+    for (int k = 0; k < QUERY_PIECES; ++k) {
+      const long long i = (block * QUERY_PIECES + k) * 256 + tid;
+      if (i < q_pieces) w[k] = q[i];
+    }
+#pragma unroll
+    for (int k = 0; k < QUERY_PIECES; ++k) {
+      const long long i = (block * QUERY_PIECES + k) * 256 + tid;
+      uint32_t* x = &w[k].x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]));
+        x[e] = pack_f16(v.x * QUERY_SCALE, v.y * QUERY_SCALE);
+      }
+      if (i < q_pieces) q_out[i] = w[k];
+    }
+    return;
+  }
   // whose tile it is: the first warp walks the requests, 32 at a time
   if (tid < 32) {
     int before = 0, seg = -1, at = 0, keys = 0;
@@ -183,7 +235,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   unsigned char* tail = gbase + (bars - base);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8 * B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * B_COUNT + 4);
-  int* tile0_slot = reinterpret_cast<int*>(tail + 8 * B_COUNT + 8);
+  Work* work = reinterpret_cast<Work*>(tail + 8 * B_COUNT + 8);
   auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -191,43 +243,33 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const int part = (int)(blockIdx.x / heads) % parts;
   const int rank = (int)(blockIdx.x / heads) / parts;
   pdl_launch_dependents();
-  int seg, r0, cnt;
-  __shared__ int tile_slot[3];
-  lse_find_tile(segment_start, num_segments, tokens_a_tile, skip_single, rank, tile_slot, seg, r0, cnt);
-  if (seg < 0) {
-    pdl_wait();
-    return;
-  }
-  const int ntok = min(tokens_a_tile, cnt - r0), nrows = ntok * group;
-  const int row_base = segment_start[seg] + r0;
-  const int pos0 = first_pos[seg] + r0;
-  const int last_pos = pos0 + ntok - 1;
-  const int n_tiles = last_pos / BN + 1;
-  const int sharing = max(1, min(parts, n_tiles / MIN_TILES_A_PART));
-  if (part >= sharing) {             // (combine works the same number out)
-    pdl_wait();
-    return;
-  }
-  const int j_lo = (int)((long long)part * n_tiles / sharing);
-  const int n_local = (int)((long long)(part + 1) * n_tiles / sharing) - j_lo;
-
   if (tid == 0) {
-    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_QC ? 2 * GROUP_THREADS : (i >= B_PF && i < B_OD) ? GROUP_THREADS : 1);
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i >= B_PF && i < B_OD ? GROUP_THREADS : 1);
     *abort_flag = 0;
     mbar_init_fence();
   }
   if (warp == MMA_WARP) tmem_alloc(tmem_slot, 512);
-  if (warp == LOADER_WARP) {
-    const int before = tiles_before(segment_start, first_pos, seg);
-    if (lane == 0) *tile0_slot = before;
-  }
+  if (warp == PV_WARP) find_work(segment_start, first_pos, num_segments, tokens_a_tile, skip_single, rank, work);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const int tile0 = *tile0_slot;
+  const int r0 = work->r0, cnt = work->rows, tile0 = work->tile0;
+  const int ntok = min(tokens_a_tile, cnt - r0), nrows = ntok * group;
+  const int row_base = work->first_row + r0;
+  const int pos0 = work->first_pos + r0;
+  const int last_pos = pos0 + ntok - 1;
+  const int n_tiles = last_pos / BN + 1;
+  const int sharing = max(1, min(parts, n_tiles / MIN_TILES_A_PART));
+  if (work->seg < 0 || part >= sharing) {      // nothing to do (how many blocks share a tile is worked out by combine as well)
+    pdl_wait();
+    if (warp == MMA_WARP) tmem_dealloc(tmem_base, 512);
+    return;
+  }
+  const int j_lo = (int)((long long)part * n_tiles / sharing);
+  const int n_local = (int)((long long)(part + 1) * n_tiles / sharing) - j_lo;
   int* const err = &lse_attn_int4_tc_error;
-  const bool held = tile0 + (first_pos[seg] + cnt + BN - 1) / BN <= capacity;   // the workspace has all of the request's tiles
+  const bool held = tile0 + (work->first_pos + cnt + BN - 1) / BN <= capacity;   // the workspace has all of the request's tiles
 
   pdl_wait();
 
@@ -255,7 +297,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   } else if (warp == MMA_WARP) {
     if (lane == 0) {
       const uint32_t idesc_s = instr_desc_f16(BM, BN, false, false);
-      bool ok = mbar_poll(bar(B_QC), 0, abort_flag, err);
+      bool ok = mbar_poll(bar(B_Q), 0, abort_flag, err);
       for (int j = 0; j < n_local && ok; ++j) {
         const int g = j & 1;
         const uint32_t parity = (uint32_t)(j >> 1) & 1u;
@@ -301,6 +343,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // ---------------------------------------------------------------- softmax
     const int g = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
+    const bool live = row < nrows;      // (the other rows hold other tokens' queries or nothing at all, and decide nothing)
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_addr = lane_addr + g * S_COLS, o_addr = lane_addr + O_COL + g * D;
     const int my_pos = pos0 + min(row, nrows - 1) / group;
@@ -312,27 +355,6 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const bool done = mbar_test(bar(which), parity) || mbar_wait(bar(which), parity, abort_flag, err);
       return __all_sync(0xffffffffu, done ? 1 : 0) != 0;
     };
-    // the queries, brought in as bfloat16, become float16 times 2^-4 where they lie; rows that no token has are zeros
-    ok = wait_all(B_Q, 0);
-    if (ok) {
-      uint4* tile = reinterpret_cast<uint4*>(gbase);
-      const int filled = tokens_a_tile * group * 8;
-      for (int i = tid; i < (int)(Q_BYTES / 16); i += 2 * GROUP_THREADS) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (i % (int)(HALF_BYTES / 16) < filled) {
-          w = tile[i];
-          uint32_t* x = &w.x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]));
-            x[e] = pack_f16(v.x * QUERY_SCALE, v.y * QUERY_SCALE);
-          }
-        }
-        tile[i] = w;
-      }
-    }
-    fence_async_smem();
-    mbar_arrive(bar(B_QC));
     for (int j = g; j < n_local && ok; j += GROUPS) {   // j counts this block's tiles
       const uint32_t parity = (uint32_t)(j >> 1) & 1u;
       ok = wait_all(B_SF + g, parity);
@@ -364,14 +386,14 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         m_used = m_seen = m_tile;
       } else {
         m_seen = fmaxf(m_seen, m_tile);
-        if (pending || __any_sync(0xffffffffu, m_tile > m_used + REDO_STEP)) {
+        if (pending || __any_sync(0xffffffffu, live && m_tile > m_used + REDO_STEP)) {
           rescale = true;
           alpha = m_used == -INFINITY ? 0.f : exp2_fast(m_used - m_seen);
           m_used = m_seen;
           l *= alpha;
         }
       }
-      pending = __any_sync(0xffffffffu, m_seen > m_used + RESCALE_STEP) != 0;
+      pending = __any_sync(0xffffffffu, live && m_seen > m_used + RESCALE_STEP) != 0;
       if (j >= GROUPS) {   // P V of this group's tile before has read the probabilities and added to O
         ok = wait_all(B_OD + g, parity ^ 1u);
         if (!ok) break;
@@ -436,40 +458,51 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int n0 = (n_local + 1) / 2, n1 = n_local / 2;     // tiles of the groups
     if (ok) ok = wait_all(B_OD + 0, (uint32_t)(n0 - 1) & 1u);
     if (ok && n1 > 0) ok = wait_all(B_OD + 1, (uint32_t)(n1 - 1) & 1u);
-    // this thread owns columns g * D / 2 .. of its row
-    const size_t out_row = (size_t)(row_base + row / group) * n_q + (head0 + head) * group + row % group;
-    float* part_row = part_o + (out_row * parts + part) * D + g * OD;
+    // This thread has columns g * D / 2 .. of its row; they go by way of the group's probability tile, which nothing reads any more, so
+    // that a warp stores whole lines (a thread its own row: 1.6 us a block).
+    const long long out_row = (long long)(row_base + row / group) * n_q + (head0 + head) * group + row % group;
     if (ok) {
       fence_after_sync();
+      unsigned char* const turn = gbase + (p_s - base) + g * P_BYTES + quarter * 8192;      // 32 rows of 256 bytes at most
+      uint4* const outs = reinterpret_cast<uint4*>(shared ? (void*)(part_o + (long long)part * D + g * OD) : (void*)(out + g * OD));
+      const int pieces = shared ? OD / 4 : OD / 8, piece_bits = 31 - __clz(pieces);       // 16 bytes each, of a row
+      const long long row_pieces = shared ? (long long)parts * (D / 4) : D / 8;
 #pragma unroll
       for (int c = 0; c < OD; c += 32) {
         uint32_t a[32], b[32];
         tmem_ld32(lane_addr + O_COL + g * OD + c, a);
         if (n1 > 0) tmem_ld32(lane_addr + O_COL + D + g * OD + c, b);
         tmem_ld_wait();
-        if (row < nrows) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v[8];
+        for (int i = 0; i < 4; ++i) {
+          float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              v[e] = __uint_as_float(a[8 * i + e]) * w0;
-              if (n1 > 0) v[e] = fmaf(__uint_as_float(b[8 * i + e]), w1, v[e]);
+          for (int e = 0; e < 8; ++e) {
+            v[e] = __uint_as_float(a[8 * i + e]) * w0;
+            if (n1 > 0) v[e] = fmaf(__uint_as_float(b[8 * i + e]), w1, v[e]);
+          }
+          uint4* const mine_row = reinterpret_cast<uint4*>(turn) + lane * pieces;
+          if (shared) {
+            const int k = c / 4 + 2 * i;
+            mine_row[k ^ (lane & 7)] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            mine_row[(k + 1) ^ (lane & 7)] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t*>(&x);
             }
-            if (shared) {
-              *reinterpret_cast<float4*>(part_row + c + 8 * i) = make_float4(v[0], v[1], v[2], v[3]);
-              *reinterpret_cast<float4*>(part_row + c + 8 * i + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                w[e] = *reinterpret_cast<const uint32_t*>(&x);
-              }
-              *reinterpret_cast<uint4*>(out + out_row * D + g * OD + c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            mine_row[(c / 8 + i) ^ (lane & 7 & (pieces - 1))] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int i = lane; i < 32 * pieces; i += 32) {
+        const int r = i >> piece_bits, k = i & (pieces - 1);
+        const long long to = __shfl_sync(0xffffffffu, out_row, r);
+        if (quarter * 32 + r < nrows) outs[to * row_pieces + k] = reinterpret_cast<const uint4*>(turn)[r * pieces + (k ^ (r & 7 & (pieces - 1)))];
       }
       if (shared && g == 0 && row < nrows) part_ml[out_row * parts + part] = make_float2(m_all, l_all);
     }
@@ -552,7 +585,7 @@ template <int D>
 int launch_portions(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* out,
                     const int* block_tables, int bt_stride, const int* segment_start, const int* first_pos, int num_segments, int tokens,
                     long long num_pages, int n_q, int n_kv, int page_size, float scale, int skip_single, int with_tiles, int capacity,
-                    int heads_at_once, int parts, void* keys, void* values, float* scratch, cudaStream_t stream) {
+                    int heads_at_once, int parts, void* keys, void* values, void* queries, float* scratch, cudaStream_t stream) {
   static SmemAllowance allowance;
   const size_t smem = attend_smem<D>();
   cudaError_t err = allow_smem(attend_int4_kernel<D>, smem, allowance);
@@ -564,14 +597,16 @@ int launch_portions(const void* q, const void* k_codes, const void* k_scales, co
   CUtensorMap map_q, map_k, map_v;
   for (int head0 = 0; head0 < n_kv; head0 += heads_at_once) {
     const int heads = n_kv - head0 < heads_at_once ? n_kv - head0 : heads_at_once;
-    if (!make_map_queries(&map_q, q, tokens, n_q, D, tokens_a_tile, group) ||
+    if (!make_map_queries(&map_q, queries, tokens, n_q, D, tokens_a_tile, group) ||
         !make_map_row_groups(&map_k, keys, (long long)heads * capacity * BN, D, BN) ||
         !make_map_row_groups(&map_v, values, (long long)heads * capacity * BN, D, BN))
       return LSE_ERR_BAD_ARGUMENT;
-    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads, BN / EXPAND_KEYS), dim3(256), 0, stream, (const unsigned char*)k_codes,
+    const long long q_pieces = head0 == 0 ? (long long)tokens * n_q * (D / 8) : 0, a_layer = (long long)capacity * heads * 256 * QUERY_PIECES;
+    if (q_pieces / a_layer > 60000) return LSE_ERR_TOO_LARGE;
+    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads, (unsigned)(BN / EXPAND_KEYS + (q_pieces + a_layer - 1) / a_layer)), dim3(256), 0, stream, (const unsigned char*)k_codes,
                      (const __nv_bfloat162*)k_scales, (const unsigned char*)v_codes, (const __nv_bfloat162*)v_scales, (uint4*)keys,
                      (uint4*)values, block_tables, bt_stride, segment_start, first_pos, num_segments, n_kv, head0, page_size,
-                     (int)num_pages, capacity, skip_single);
+                     (int)num_pages, capacity, skip_single, (const uint4*)q, (uint4*)queries, q_pieces);
     if (err != cudaSuccess) return (int)err;
     err = lse_launch(attend_int4_kernel<D>, dim3((unsigned)((long long)tiles * heads * parts)), dim3(THREADS), smem, stream, map_q, map_k,
                      map_v, (__nv_bfloat16*)out, segment_start, first_pos, num_segments, n_q, group, heads, head0, tokens_a_tile,
@@ -605,23 +640,23 @@ extern "C" int lse_attention_int4_tc_status_reset(void) {
 // q, out bfloat16 [tokens, n_q, head_dim]; the cache as int4_cache.cu leaves it; segment_start [S + 1]: first row of each request's
 // portion, first_pos [S]: that row's position.  keys, values: float16 [heads_at_once, capacity * 128, head_dim], capacity = tiles of 128
 // keys of all requests together, each request's rounded up (rows of a request that does not fit come out as NaN).  with_tiles: requests
-// that have rows here, at most.  parts > 1 (at most 8): scratch holds tokens * n_q * parts * (head_dim + 2) float32.
+// that have rows here, at most.  queries: float16 [tokens, n_q, head_dim].  parts > 1 (at most 8): scratch holds tokens * n_q * parts * (head_dim + 2) float32.
 extern "C" int lse_paged_attention_prefill_int4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                                                 const void* v_scales, void* out, const int* block_tables, int bt_stride,
                                                 const int* segment_start, const int* first_pos, int num_segments, int tokens,
                                                 long long num_pages, int n_q, int n_kv, int head_dim, int page_size, float scale,
                                                 int skip_single, int with_tiles, int capacity, int heads_at_once, int parts, void* keys,
-                                                void* values, float* scratch, cudaStream_t stream) {
+                                                void* values, void* queries, float* scratch, cudaStream_t stream) {
   if (tokens <= 0 || num_segments <= 0) return 0;
   if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_q % n_kv || n_q / n_kv > BM || page_size <= 0 || num_pages <= 0 ||
       num_pages * page_size > 0x7fffffffLL || !(scale > 0.f) || capacity < 1 || heads_at_once < 1 || parts < 1 || parts > MAX_PARTS ||
-      with_tiles < 1 || keys == nullptr || values == nullptr || (parts > 1 && scratch == nullptr) ||
+      with_tiles < 1 || keys == nullptr || values == nullptr || queries == nullptr || (parts > 1 && scratch == nullptr) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales |
-        (uintptr_t)keys | (uintptr_t)values | (uintptr_t)scratch) & 15))
+        (uintptr_t)keys | (uintptr_t)values | (uintptr_t)queries | (uintptr_t)scratch) & 15))
     return LSE_ERR_BAD_ARGUMENT;
   if (heads_at_once > 65535 || (long long)heads_at_once * capacity * (BN / 8) > 0x7fffffffLL) return LSE_ERR_TOO_LARGE;
 #define LSE_INT4_ARGS q, k_codes, k_scales, v_codes, v_scales, out, block_tables, bt_stride, segment_start, first_pos, num_segments, \
-  tokens, num_pages, n_q, n_kv, page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts, keys, values, scratch, stream
+  tokens, num_pages, n_q, n_kv, page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts, keys, values, queries, scratch, stream
   return head_dim == 128 ? launch_portions<128>(LSE_INT4_ARGS) : launch_portions<64>(LSE_INT4_ARGS);
 #undef LSE_INT4_ARGS
 }

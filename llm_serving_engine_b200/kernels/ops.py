@@ -2323,16 +2323,17 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     # several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs
     blocks = (-(-tokens // (INT4_TILE // group)) + with_tiles) * heads_at_once
     parts = max(1, min(8, 5 * sm_count() // (4 * blocks)))
-    # float16 keys, float16 values, and (several parts) float32 outputs, maxima and sums of every part
+    # float16 keys, values and queries, and (several parts) float32 outputs, maxima and sums of every part
     halves = heads_at_once * a_head
-    workspace = torch.empty(4 * halves + (4 * tokens * n_q * parts * (dim + 2) if parts > 1 else 0), dtype=_U8, device=q.device)
+    queries = tokens * n_q * dim
+    workspace = torch.empty(4 * halves + 2 * queries + (4 * tokens * n_q * parts * (dim + 2) if parts > 1 else 0), dtype=_U8, device=q.device)
     at = workspace.data_ptr()
     check(library.load().lse_paged_attention_prefill_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                                           v_scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), table_stride,
                                                           segment_start.data_ptr(), segment_first_position.data_ptr(), segments,
                                                           tokens, pages, n_q, n_kv, dim, page_size, scale, skip_single, with_tiles,
-                                                          capacity, heads_at_once, parts, at, at + 2 * halves,
-                                                          at + 4 * halves if parts > 1 else None, _current_stream(device)), name)
+                                                          capacity, heads_at_once, parts, at, at + 2 * halves, at + 4 * halves,
+                                                          at + 4 * halves + 2 * queries if parts > 1 else None, _current_stream(device)), name)
     return out
 
 
