@@ -467,3 +467,49 @@ def test_write_of_rows_on_the_borders_of_rounding(dim, pairing):
         u, s, c = plain.quantise(rows.to(D64).cuda())
         assert torch.equal(scales[page, :, at], torch.stack([s, c], -1).bfloat16())
         assert torch.equal(codes[page, :, at], plain.pack(u))
+
+
+def test_portions_of_many_requests():
+    """More requests than a warp has lanes, with none, one or many rows."""
+    counts = [(s * 7) % 23 if s % 5 else s % 2 for s in range(75)]
+    firsts = [(s * 37) % 190 for s in range(75)]
+    g, cache, tables, start, first = portion_case(counts, firsts, 2, 64, 16, 9)
+    tokens = sum(counts)
+    q = torch.randn((tokens, 10, 64), generator=g).bfloat16().cuda()
+    for singles in (False, True):
+        out = torch.full_like(q, 3.0)
+        ops.paged_attention_prefill_int4(q, *cache, out, tables, start, first, 0.125, keys=tokens + sum(firsts), skip_single=singles)
+        assert portions(cache, tables, counts, firsts, q, out, 0.125, 16, singles) > 200
+        if singles:
+            alone = torch.tensor([n == 1 for n in counts for _ in range(n)]).cuda()
+            assert (out[alone] == 3.0).all() and alone.any()
+
+
+@pytest.mark.parametrize("splits", [2, 24])
+def test_rows_of_many_requests(splits):
+    """More rows than a block has threads, padding and empty rows among them."""
+    g = torch.Generator().manual_seed(12)
+    rows = 300
+    cache = fill_cache(g, 4 * rows, 1, 16, 64)
+    tables = torch.randperm(4 * rows, generator=g).int().view(rows, 4).cuda()
+    positions = torch.randint(0, 64, (rows,), generator=g)
+    positions[::17] = -1
+    segments = torch.randperm(rows, generator=g)
+    segments[5::31] = -1
+    q = torch.randn((rows, 3, 64), generator=g).bfloat16().cuda()
+    out = torch.full_like(q, 3.0)
+    ops.paged_attention_decode_int4(q, *cache, out, tables, segments.int().cuda(), positions.int().cuda(), 0.125, num_splits=splits)
+    for row, (segment, position) in enumerate(zip(segments.tolist(), positions.tolist())):
+        if segment < 0:
+            assert (out[row] == 3.0).all()
+        elif position < 0:
+            assert (out[row] == 0.0).all()
+        else:
+            k, v = request_rows(cache, tables[segment], position + 1, 16)
+            expected, weighed = plain.attend(q[row], k, v, position, 0.125)
+            # What is rounded to bfloat16 (2^-8) is weight times scale, of which a value takes u - 8: a term is off by 2^-8 of the value's
+            # distance from its row's centre, which with few keys is more than 2^-8 of the value where the two have other signs.
+            pages = tables[segment, :position // 16 + 1].long()
+            centre = cache[3][pages][..., 1].to(D64).transpose(1, 2).flatten(0, 1)[:position + 1, :, None]
+            _, apart = plain.attend(q[row], k, v - centre, position, 0.125)
+            assert ((out[row].to(D64) - expected).abs() <= bound(expected, apart) + 2.0 ** -14 * weighed).all(), row
