@@ -6,16 +6,21 @@
 // round them to bfloat16 and cost a multiply-add a value.)
 //
 // One block = (row, up to 8 query heads of a key/value head, a part of the keys); its warps take tiles of 16 keys in turn.  Keys ride the
-// M side of mma.sync m16n8k16, heads the N side (S^T = K Q^T, O^T = V^T P^T).  Codes go from global memory straight into the
-// registers that the instruction wants them in: which d a thread holds where is free as long as q, or the output, follows, so
+// M side of mma.sync m16n8k16, heads the N side (S^T = K Q^T, O^T = V^T P^T).  Every warp keeps a ring of tiles of its own, as they lie in
+// the cache, filled by cp.async, and reads them into the registers that the instruction wants them in: which d a thread holds
+// where is free as long as q, or the output, follows, so
 //   keys    lane 4 g + t reads D / 8 consecutive bytes of keys g and g + 8: its d are t D / 4 .. ;
 //   values  lane 4 g + t reads D / 16 consecutive bytes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: its d are g D / 8 .. .
-// Each warp load covers whole 64-byte rows.  Two nibbles 16 bits apart become a pair of bfloat16 by one shift and one and-or.  For
+// Two nibbles 16 bits apart become a pair of bfloat16 by one shift and one and-or.  For
 // keys that is 16 + u, and the accumulators start at -24 sum(q); float32 rounds sums of 24 |q| instead of 8 |q| then, which is far
 // below the rounding of a probability.  Values lose the offset by a subtraction, which is exact: sums of
 // values run over the whole context, and an offset there would cost what the result loses by averaging.
 // Softmax in base two, float32; the maximum in use is raised only when a score outgrows it by 2^8 (the sums carry the same
-// factor, so the quotient is exact either way).  Probabilities are rounded to bfloat16 for the second product, as everywhere here.
+// factor, so the quotient is exact either way).  What is rounded to bfloat16 for the second product is a probability times its
+// value's scale: a term is off by 2^-9 of s (u - 8), a sixty-fourth of a step of the codes at most.
+// What bounds it: a row's chain of waits (positions, block table, tiles, the parts' meeting), then a warp's chain of some 200
+// instructions a tile.  64 rows of 12 / 2 heads of 128 over 950 to 2,850 keys (33.5 MB): 15.4 us; one row of 28 / 4 heads over 30,000
+// keys (16.3 MB): 13.5 us, 4 of them the second launch.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

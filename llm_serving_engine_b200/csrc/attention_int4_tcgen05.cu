@@ -7,7 +7,8 @@
 //             read them.  Float16 because a value s (u - 8) + c rounded to bfloat16 would be off by up to 2^-8, as much as the result's own
 //             rounding, and float16 by 2^-11; keys are scaled by 2^-8 and queries by 2^-4 (exact), which keeps scores of
 //             keys up to 2^24 in range.  A row that float16 does not hold, or that is not a number, becomes NaN in its key and
-//             zeros in its value: who attends to it gets NaN, and nobody else does.
+//             zeros in its value: who attends to it gets NaN, and nobody else does.  The queries become float16 here as well (in
+//             attend every block's tensor cores waited 0.9 us for it).
 //   attend    one block = 128 score rows of one request and key/value head: (token, query head of the group) pairs, so that
 //             keys are brought in once for all heads of a group and portions of a few tokens fill the rows.  Keys are walked in tiles
 //             of 128, which go alternately to two groups of four softmax warps, each with its own key and value stage, accumulators in
@@ -19,8 +20,12 @@
 //                             when a maximum has grown by more than 2^8 (at once beyond 2^14: float16 ends at 2^16).
 //   combine   with fewer blocks than SMs, several blocks share the keys of a tile; each leaves its part in a workspace of this
 //             call, and another launch adds them up, in the order of the parts.
-// What bounds attend: the softmax threads' instructions and exponentials (128 x 128 exponentials a tile at 16 a cycle, and the
-// tensor cores take as long for the tile's two products).
+// What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s: tensor cores busy for 58% of
+// the cycles, the unit of the exponentials for 58% (128 x 128 a tile at 16 a cycle), and 656 blocks leave a fifth turn of
+// the SMs half empty.  All exponentials of a tile before the wait for the product of the tile before: 328 us.  Small launches: a
+// block's way from its start to its first scores (2.7 us), through a tile and to its end is 8 us, and eight portions of
+// about 200 rows (160 blocks, 24.4 us) make some SMs go it twice; starting the blocks with most keys first did not help (the
+// search for them cost 1.6 us a block).
 // Every wait is bounded (see tcgen05.cuh); a block whose wait gave up leaves NaN in its rows, frees its tensor memory and returns.
 #include <cuda_fp16.h>
 

@@ -2220,8 +2220,8 @@ INT4_DECODE_BLOCKS = 4          # blocks that an SM holds
 INT4_DECODE_WARPS = 4           # warps of a block, which take tiles of 16 keys in turn
 INT4_DECODE_CLUSTER = 8         # most blocks that share a row's keys in one launch
 # Tiles of a warp beyond which all rows' tiles are cut into equal runs: with contexts from a half to one and a half times 1,900, 64
-# rows of 12 / 2 heads (11 tiles) take 16.6 us in one launch and 18 to 20 in runs, with 6,000, 16 rows of 8 heads of 64 (35 tiles) 27
-# and 23; one row of 28 / 4 heads over 30,000 keys 31 and 12.
+# rows of 12 / 2 heads (11 tiles) take 15.4 us in one launch and 18 to 20 in runs, with 6,000, 16 rows of 8 heads of 64 (35 tiles) 27
+# and 23; one row of 28 / 4 heads over 30,000 keys 31 and 13.5.
 INT4_DECODE_TILES = 14
 
 
