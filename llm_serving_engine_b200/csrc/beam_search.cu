@@ -11,11 +11,12 @@
 // merge: a block per request, from the chunks' leavings.  Offers are compared in 64 bits: two beams' offers can be closer than
 // float32 tells apart, and lse's error would decide.
 // What bounds the choice: the logits are read once, 4 bytes each.  256 rows of 151,936 (32 requests of 8 beams, 156 MB) take 36 us for
-// both launches, 4.3 TB/s: the second turn of the SMs' blocks ends unevenly, and merge is 4 us; 4 rows 8.5 us, most of it the two
+// both launches, 4.3 TB/s: the second turn of the SMs' blocks ends unevenly, and merge is 4 us; 4 rows 9.1 us, most of it the two
 // launches' latencies.  Pieces of twice the length 37 to 40 us, one more block an SM 38, loads past the L1 44.
 //
 // The last kernels of a step: the next step's read its metadata (token ids, block tables) before they wait for the kernels before
-// them.  So the kernels here that write metadata never let the next one start early.
+// them.  So the kernels here that write metadata never let the next one start early, and their threads end only when what they wrote is
+// visible to the whole device.
 #include "common.cuh"
 
 namespace {
@@ -344,6 +345,7 @@ beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
       if (rank < beams) put(rank, list_v[i], list_at[i]);
     }
     for (int i = found + tid; i < beams; i += MERGE_THREADS) nothing(i);
+    if (tid < max(found, beams)) __threadfence();      // (whoever may have written)
     return;
   }
   // more ties than the list has room for: one by one
@@ -374,6 +376,7 @@ beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
       if (win_v[w] > last_v || (win_v[w] == last_v && win_at[w] < last_at)) { last_v = win_v[w]; last_at = win_at[w]; }
     if (tid == 0) { if (last_v > -INFINITY) put(k, last_v, last_at); else nothing(k); }
   }
+  if (tid == 0) __threadfence();
 }
 
 // ------------------------------------------------------------------ after the choice
@@ -383,7 +386,7 @@ beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
 // the parent was filling; every further child takes that of a beam without a child (there are as many of either), and the
 // parent's page is copied into it.  No page is read that another child's copy writes, so the copies need no order.
 // What bounds it: the bytes of the pages that have to be copied, read and written once (16 requests of 8 beams, 28 layers of 4 heads of
-// 128 in bfloat16: 77 MB in 17.8 us, 4.4 TB/s), or the launch where there are few (2.8 us).
+// 128 in bfloat16: 77 MB in 18 to 21 us, 3.7 to 4.4 TB/s), or the launch where there are few (2.9 us).
 constexpr int MAX_STORAGES = 24;
 // A page's words (of sizeof V) are copied in pieces of PIECE; 1 << lane_bits threads take a piece's words, the rest of a block's further
 // outer parts; `items` pieces for the whole storage.
@@ -419,6 +422,7 @@ beam_reorder_kernel(const int* parents, int beams, const int* tables, int table_
   if (blockIdx.y == 0 && new_tables != nullptr)
     for (int i = threadIdx.x; i < width; i += blockDim.x)
       new_tables[(size_t)row * new_stride + i] = i < full ? from[i] : (i == full && filling) ? target : own[i];
+  if (blockIdx.y == 0) __threadfence();
   if (!copies || !filling) return;
   for (int k = 0; k < storages.n; ++k) {
     const Storage& s = storages.s[k];

@@ -5,7 +5,8 @@
 // Request s brings counts[s] tokens behind first[s] earlier ones and owns pages[page_start[s] .. page_start[s + 1]).  Every block
 // of the rows adds up all counts itself, 256 at a time (a step holds hundreds of requests at most), and looks its rows up in the
 // running sums, so one launch does it: what bounds it is the launch and two dependent loads, not the few hundred KB written.
-// The step's kernels read this metadata before they wait for the kernels before them, so this one never lets the next start early.
+// The step's kernels read this metadata before they wait for the kernels before them, so this one never lets the next start early, and
+// its threads end only when what they wrote is visible to the whole device.
 #include "common.cuh"
 
 namespace {
@@ -26,6 +27,7 @@ step_tables_kernel(const int* first, const int* counts, const int* pages,
     if (s >= requests) return;
     const int lo = page_start[s], hi = page_start[s + 1];
     tables[(size_t)s * table_stride + i] = i < hi - lo ? pages[lo + i] : -1;
+    __threadfence();
     return;
   }
   const int row = (int)blockIdx.x * THREADS + tid;
@@ -48,6 +50,7 @@ step_tables_kernel(const int* first, const int* counts, const int* pages,
       segment_start[s] = before + sum - mine;
       contexts[s] = first[s] + mine;
       if (s == requests - 1) segment_start[requests] = before + sum;
+      __threadfence();
     }
     __syncthreads();
     const int last = ends[THREADS - 1];
@@ -74,6 +77,7 @@ step_tables_kernel(const int* first, const int* counts, const int* pages,
   segment_of_token[row] = seg;
   positions[row] = position;
   slots[row] = slot;
+  __threadfence();
 }
 
 }  // namespace
