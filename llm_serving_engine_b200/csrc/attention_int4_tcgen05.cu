@@ -22,7 +22,8 @@
 //             call, and another launch adds them up, in the order of the parts.
 // What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s: tensor cores busy for 58% of
 // the cycles, the unit of the exponentials for 58% (128 x 128 a tile at 16 a cycle), and 656 blocks leave a fifth turn of
-// the SMs half empty.  All exponentials of a tile before the wait for the product of the tile before: 328 us.  Small launches: a
+// the SMs half empty.  All exponentials of a tile before the wait for the product of the tile before: 328 us, a quarter of them:
+// 320; a quarter of the exponentials by a polynomial instead: 335; scores read twice from tensor memory, 32 at a time: 335.  Small launches: a
 // block's way from its start to its first scores (2.7 us), through a tile and to its end is 8 us, and eight portions of
 // about 200 rows (160 blocks, 24.4 us) make some SMs go it twice; starting the blocks with most keys first did not help (the
 // search for them cost 1.6 us a block).
@@ -271,8 +272,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (warp == MMA_WARP) tmem_dealloc(tmem_base, 512);
     return;
   }
-  const int j_lo = (int)((long long)part * n_tiles / sharing);
-  const int n_local = (int)((long long)(part + 1) * n_tiles / sharing) - j_lo;
+  const int j_lo = sharing == 1 ? 0 : part * n_tiles / sharing, n_local = sharing == 1 ? n_tiles : (part + 1) * n_tiles / sharing - j_lo;
   int* const err = &lse_attn_int4_tc_error;
   const bool held = tile0 + (work->first_pos + cnt + BN - 1) / BN <= capacity;   // the workspace has all of the request's tiles
 

@@ -11,12 +11,12 @@
 // merge: a block per request, from the chunks' leavings.  Offers are compared in 64 bits: two beams' offers can be closer than
 // float32 tells apart, and lse's error would decide.
 // What bounds the choice: the logits are read once, 4 bytes each.  256 rows of 151,936 (32 requests of 8 beams, 156 MB) take 36 us for
-// both launches, 4.3 TB/s: the second turn of the SMs' blocks ends unevenly, and merge is 4 us; 4 rows 9.1 us, most of it the two
+// both launches, 4.3 TB/s: the second turn of the SMs' blocks ends unevenly, and merge is 4 us; 4 rows 8.9 us, most of it the two
 // launches' latencies.  Pieces of twice the length 37 to 40 us, one more block an SM 38, loads past the L1 44.
 //
-// The last kernels of a step: the next step's read its metadata (token ids, block tables) before they wait for the kernels before
-// them.  So the kernels here that write metadata never let the next one start early, and their threads end only when what they wrote is
-// visible to the whole device.
+// The last kernels of a step: the next step's read its block tables before they wait for the kernels before them (scores, tokens and parents
+// after that).  So merge and reorder never let the next kernel start early, and reorder's threads end only when the tables that they
+// wrote are visible to the whole device.
 #include "common.cuh"
 
 namespace {
@@ -345,7 +345,6 @@ beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
       if (rank < beams) put(rank, list_v[i], list_at[i]);
     }
     for (int i = found + tid; i < beams; i += MERGE_THREADS) nothing(i);
-    if (tid < max(found, beams)) __threadfence();      // (whoever may have written)
     return;
   }
   // more ties than the list has room for: one by one
@@ -376,7 +375,6 @@ beam_merge_kernel(const Best* best, const Sum* sums, int chunks, int beams,
       if (win_v[w] > last_v || (win_v[w] == last_v && win_at[w] < last_at)) { last_v = win_v[w]; last_at = win_at[w]; }
     if (tid == 0) { if (last_v > -INFINITY) put(k, last_v, last_at); else nothing(k); }
   }
-  if (tid == 0) __threadfence();
 }
 
 // ------------------------------------------------------------------ after the choice
