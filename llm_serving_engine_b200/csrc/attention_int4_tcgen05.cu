@@ -20,13 +20,13 @@
 //                             when a maximum has grown by more than 2^8 (at once beyond 2^14: float16 ends at 2^16).
 //   combine   with fewer blocks than SMs, several blocks share the keys of a tile; each leaves its part in a workspace of this
 //             call, and another launch adds them up, in the order of the parts.
-// What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s: tensor cores busy for 58% of
-// the cycles, the unit of the exponentials for 58% (128 x 128 a tile at 16 a cycle), and 656 blocks leave a fifth turn of
-// the SMs half empty.  All exponentials of a tile before the wait for the product of the tile before: 328 us, a quarter of them:
-// 320; a quarter of the exponentials by a polynomial instead: 335; scores read twice from tensor memory, 32 at a time: 335.  Small launches: a
-// block's way from its start to its first scores (2.7 us), through a tile and to its end is 8 us, and eight portions of
-// about 200 rows (160 blocks, 24.4 us) make some SMs go it twice; starting the blocks with most keys first did not help (the
-// search for them cost 1.6 us a block).
+// What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s (324 at the power cap): tensor
+// cores busy for 58% of the cycles, the unit of the exponentials for 58% (128 x 128 a tile at 16 a cycle), and 656 blocks leave a
+// fifth turn of the SMs half empty.  Side by side, 324: all exponentials of a tile before the wait for the product of the tile
+// before 350, a quarter of them 338; a quarter of the exponentials by a polynomial 361; scores read twice from tensor memory, 32 at a
+// time, 354.  Small launches: a block's way from its start to its first scores (2.7 us), through a few tiles and to its end is 8 us,
+// and eight portions of about 200 rows (160 blocks, 24.1 us) make some SMs go it twice; starting the blocks with most keys first
+// took 26.6 (the search for them costs every block more than the order wins).
 // Every wait is bounded (see tcgen05.cuh); a block whose wait gave up leaves NaN in its rows, frees its tensor memory and returns.
 #include <cuda_fp16.h>
 
