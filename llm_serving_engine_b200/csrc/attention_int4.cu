@@ -17,7 +17,7 @@
 // values run over the whole context, and an offset there would cost what the result loses by averaging.
 // Softmax in base two, float32; the maximum in use is raised only when a score outgrows it by 2^8 (the sums carry the same
 // factor, so the quotient is exact either way).  What is rounded to bfloat16 for the second product is a probability times its
-// value's scale: a term is off by 2^-9 of s (u - 8), a sixty-fourth of a step of the codes at most.
+// value's scale: a term is off by 2^-8 of s (u - 8), a thirty-second of a step of the codes at most.
 // What bounds it: a row's chain of waits (positions, block table, tiles, the parts' meeting), then instructions, some 400 a warp and tile
 // all told (half of them make bfloat16 of the codes).  64 rows of 12 / 2 heads of 128 over 950 to 2,850 keys (33.5 MB): 15.4 us, over
 // 2,000 each 13.8 (24.1 over bfloat16 pages); 16 rows over 8,000: 17.7 (24.0); one row of 28 / 4 heads over 30,000 keys (16.3 MB): 13.5 us
