@@ -2414,6 +2414,8 @@ def beam_reorder(parents: torch.Tensor, block_tables: torch.Tensor, lengths: tor
     if (len(shape) != 2 or block_tables.dtype is not _I32 or new_tables.dtype is not _I32 or shape[0] != requests * beams or shape[1] == 0
             or new_tables.shape != shape or strides[1] != 1 or new_strides[1] != 1):
         _refuse(name, "block tables are int32 [requests * beams, pages]")
+    if shape[0] > 1 and new_strides[0] < shape[1]:
+        _refuse(name, "rows of the new tables overlap")
     tables_at, new_at = block_tables.data_ptr(), new_tables.data_ptr()
     if tables_at == new_at:
         _refuse(name, "the new tables are made in another tensor than the old ones")
@@ -2485,6 +2487,8 @@ def step_tables(first: torch.Tensor, counts: torch.Tensor, pages: torch.Tensor, 
     shape, strides = block_tables.shape, block_tables.stride()
     if block_tables.dtype is not _I32 or len(shape) != 2 or shape[0] != requests or strides[1] != 1:
         _refuse(name, "block tables are int32 [requests, pages]")
+    if requests > 1 and strides[0] < shape[1]:
+        _refuse(name, "rows of the block tables overlap")
     if not first.is_cuda:
         _need_cuda(first)
     device = _get_device()
@@ -2496,4 +2500,4 @@ def step_tables(first: torch.Tensor, counts: torch.Tensor, pages: torch.Tensor, 
     check(library.load().lse_step_tables(first.data_ptr(), counts.data_ptr(), pages.data_ptr(), page_start.data_ptr(), requests,
                                          page_size, tokens, segment_start.data_ptr(), segment_of_token.data_ptr(),
                                          positions.data_ptr(), slot_mapping.data_ptr(), contexts.data_ptr(), block_tables.data_ptr(),
-                                         max(width, strides[0]), width, _current_stream(device)), name)
+                                         strides[0] if requests > 1 else width, width, _current_stream(device)), name)
