@@ -694,9 +694,11 @@ extern "C" int lse_paged_attention_decode_int4(const void* q, const void* k_code
                                                float scale, int splits, int runs,
                                                long long num_pages, int num_segments, cudaStream_t stream) {
   if (tokens <= 0) return 0;
+  const int unit = page_size <= 0 ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 1;
   if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_q % n_kv || page_size <= 0 || num_pages <= 0 || splits < 1 || runs < 0 ||
       num_pages * page_size > 0x7fffffffLL || (runs > 0 && scratch == nullptr) ||
-      (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales | (uintptr_t)scratch) & 15))
+      (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)scratch) & 15) ||
+      (((uintptr_t)k_scales | (uintptr_t)v_scales) & (unit > 1 ? 15 : 3)))      // scales come four rows at a time, or row by row
     return LSE_ERR_BAD_ARGUMENT;
   if (num_pages * page_size / 8 * n_kv > 0xffffffffLL || n_q > 65535 ||
       (long long)tokens * (((long long)bt_stride * page_size + TILE - 1) / TILE) * n_kv * ((n_q / n_kv + HEADS - 1) / HEADS) > 0x7fffffffLL) return LSE_ERR_TOO_LARGE;
@@ -706,7 +708,6 @@ extern "C" int lse_paged_attention_decode_int4(const void* q, const void* k_code
     for (cache.pm.shift = 0; 1 << cache.pm.shift < page_size;) ++cache.pm.shift;
   const Rows rows = {segment_of_token, positions, segment_start};
 #define LSE_INT4_ARGS q, cache, out, scratch, block_tables, bt_stride, rows, tokens, n_q, scale, splits, runs, num_segments, stream
-  const int unit = page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 1;
   if (head_dim == 128) return unit == 16 ? launch_rows<128, 16>(LSE_INT4_ARGS) : unit == 8 ? launch_rows<128, 8>(LSE_INT4_ARGS) : launch_rows<128, 1>(LSE_INT4_ARGS);
   return unit == 16 ? launch_rows<64, 16>(LSE_INT4_ARGS) : unit == 8 ? launch_rows<64, 8>(LSE_INT4_ARGS) : launch_rows<64, 1>(LSE_INT4_ARGS);
 #undef LSE_INT4_ARGS

@@ -656,8 +656,8 @@ extern "C" int lse_paged_attention_prefill_int4(const void* q, const void* k_cod
   if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_q % n_kv || n_q / n_kv > BM || page_size <= 0 || num_pages <= 0 ||
       num_pages * page_size > 0x7fffffffLL || !(scale > 0.f) || capacity < 1 || heads_at_once < 1 || parts < 1 || parts > MAX_PARTS ||
       with_tiles < 1 || keys == nullptr || values == nullptr || queries == nullptr || (parts > 1 && scratch == nullptr) ||
-      (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales |
-        (uintptr_t)keys | (uintptr_t)values | (uintptr_t)queries | (uintptr_t)scratch) & 15))
+      (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)keys | (uintptr_t)values |
+        (uintptr_t)queries | (uintptr_t)scratch) & 15) || (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3))
     return LSE_ERR_BAD_ARGUMENT;
   if (heads_at_once > 65535 || (long long)heads_at_once * capacity * (BN / 8) > 0x7fffffffLL) return LSE_ERR_TOO_LARGE;
 #define LSE_INT4_ARGS q, k_codes, k_scales, v_codes, v_scales, out, block_tables, bt_stride, segment_start, first_pos, num_segments, \

@@ -328,8 +328,8 @@ extern "C" int lse_rope_kv_write_int4(const void* qkv, int in_dtype, int n_parti
   const int align = in_dtype == LSE_DTYPE_F32 ? 15 : 7;
   if (bad_cache(n_kv, head_dim, page_size, num_pages) || n_q <= 0 || (pairing != 0 && pairing != 1) || n_partials < 1 ||
       qkv_stride % 4 || partial_stride % 4 || ((uintptr_t)qkv & align) ||
-      (((uintptr_t)bias | (uintptr_t)inv_freq | (uintptr_t)q_out | (uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes |
-        (uintptr_t)v_scales) & 15))
+      (((uintptr_t)bias | (uintptr_t)inv_freq | (uintptr_t)q_out | (uintptr_t)k_codes | (uintptr_t)v_codes) & 15) ||
+      (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3))      // (a layer's parts of a cache whose pages are no multiple of four rows)
     return LSE_ERR_BAD_ARGUMENT;
 #define LSE_INT4_ARGS qkv, n_partials, partial_stride, bias, positions, slot_mapping, inv_freq, q_out, k_codes, k_scales, v_codes, \
   v_scales, tokens, n_q, n_kv, page_size, pairing, qkv_stride, num_pages * page_size, stream
@@ -347,7 +347,8 @@ extern "C" int lse_kv_read_int4(const void* k_codes, const void* k_scales, const
                                 int page_size, long long num_pages, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (bad_cache(n_kv, head_dim, page_size, num_pages) ||
-      (((uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales | (uintptr_t)k_out | (uintptr_t)v_out) & 15))
+      (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15) ||
+      (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3))
     return LSE_ERR_BAD_ARGUMENT;
   const long long items = (long long)tokens * n_kv * (head_dim / 8);
   const dim3 grid((unsigned)((items + 255) / 256), 2);
