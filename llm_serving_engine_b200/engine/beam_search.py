@@ -45,7 +45,8 @@ class BeamSearch:
         self.use_graph = runner.use_graphs if use_graph is None else use_graph
 
     def search(self, prompts: list[list[int]], max_new_tokens: int) -> list[list[Beam]]:
-        """The best ``beams`` continuations of every prompt, the best first."""
+        """The best ``beams`` continuations of every prompt, the best first (fewer where the model's logits leave fewer).  Raises
+        ``KernelError`` when a kernel's bounded wait gave up meanwhile, or no beam of a prompt is left."""
         runner, cache = self.runner, self.runner.cache
         if not prompts or max_new_tokens <= 0:
             raise ValueError("a search needs prompts and a positive max_new_tokens")
@@ -61,6 +62,10 @@ class BeamSearch:
                 cache.create(name)
             logits = torch.stack([self._prompt(name, prompt) for name, prompt in zip(names, prompts)])
             return self._beams(names, [len(prompt) for prompt in prompts], logits, max_new_tokens)
+        except BaseException:
+            torch.cuda.current_stream().synchronize()
+            ops.kernel_status_reset()        # what this search's kernels left does not fail the next steps
+            raise
         finally:
             torch.cuda.current_stream().synchronize()
             for name in names:
@@ -102,17 +107,26 @@ class BeamSearch:
         scores = torch.full((requests, beams), -torch.inf, dtype=torch.float32, device=device)
         scores[:, 0] = 0.0
         held.scores.copy_(scores)
-        chosen = []
+        chosen, status = [], ops.kernel_status_words()
         step = _Step(held, self.end_token, self.use_graph and max_new_tokens > 3)
         logits = logits.repeat_interleave(beams, 0)
         for index in range(max_new_tokens):
             chosen.append(step.choose(logits))
             if index + 1 < max_new_tokens:
                 logits = step.run()
-            if index % 16 == 15 and bool(held.ended.all()):      # (a look at the device now and then)
-                break
-        return self._traced([[part.tolist() for part in pair] for pair in torch.stack(chosen).cpu()], held.scores.cpu().tolist(),
-                            held.ended.cpu().tolist())
+            if index % 16 == 15:                # (a look at the device now and then)
+                ops.kernel_status_async(status)
+                over = bool(held.ended.all())
+                ops.kernel_status_check(status)
+                if over:
+                    break
+        ops.kernel_status_async(status)         # arrives with what was chosen
+        chosen, scores, ended = torch.stack(chosen).cpu(), held.scores.cpu().tolist(), held.ended.cpu().tolist()
+        ops.kernel_status_check(status)
+        found = self._traced([[part.tolist() for part in pair] for pair in chosen], scores, ended)
+        if not all(found):
+            raise ops.KernelError(f"prompt {found.index([])}: the model's logits are not numbers, no beam is left")
+        return found
 
     def _traced(self, chosen, scores, ended) -> list[list[Beam]]:
         found = []

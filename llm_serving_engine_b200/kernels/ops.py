@@ -673,6 +673,8 @@ def gemm_bf16_skinny_status() -> int:
 _STATUS_WORDS = (("gemm_tcgen05", "lse_gemm_bf16_skinny_status"), ("attention_tcgen05", "lse_attention_tc_status"),
                  ("attention_expanded_tcgen05", "lse_attention_expanded_status"), ("decode_layers", "lse_decode_layers_status"),
                  ("gemm_pairs", "lse_gemm_pairs_status"), ("attention_int4_tcgen05", "lse_attention_int4_tc_status"))
+_STATUS_NAMES = ("the few-rows product", "the tcgen05 prompt attention", "the attention over expanded latents", "the decode step",
+                 "the product on pairs of SMs", "the attention over 4-bit keys")
 
 
 def kernel_status_async(host_words: torch.Tensor) -> None:
@@ -701,6 +703,26 @@ def kernel_status_reset() -> None:
             getattr(lib, entry + "_reset")()
     for _, counters in _ATTENTION_TC_SCRATCH.values():   # a block that gave up may have left its arrival uncounted
         counters.zero_()
+
+
+def kernel_status_words() -> torch.Tensor:
+    """A pinned buffer for :func:`kernel_status_async`, a word for every kernel."""
+    return torch.zeros(len(_STATUS_WORDS), dtype=torch.int32, pin_memory=True)
+
+
+def kernel_status_check(host_words: torch.Tensor) -> None:
+    """Raises, once the copies that :func:`kernel_status_async` queued have arrived, if a kernel's wait gave up, and clears the words
+    on the host and on the device: the failure is reported once, and belongs to the steps that it spoilt."""
+    words = host_words.tolist()
+    if not any(words):
+        return
+    host_words.zero_()
+    kernel_status_reset()
+    if len(words) > 2 and words[2] == EXPANDED_ROWS_LEFT_OUT:
+        raise KernelError("the attention over expanded latents was given room for fewer rows than the requests hold: "
+                          "the step's results are not valid")
+    which = " and ".join(name for name, word in zip(_STATUS_NAMES, words) if word)
+    raise KernelError(f"a bounded wait inside {which} gave up: the step's results are not valid")
 
 
 def decode_layers_supported(layers: int, rows: int, hidden: int, inter: int, n_q: int, n_kv: int, vocab: int) -> bool:

@@ -54,7 +54,7 @@ class _Turn:
         self.dev_i = torch.empty((2, max_rows), dtype=torch.int64, device=device)
         self.out = torch.empty(max_rows, dtype=torch.int32, device=device)
         self.host_out = torch.empty(max_rows, dtype=torch.int32, pin_memory=pinned)
-        self.host_status = torch.zeros(6, dtype=torch.int32, pin_memory=pinned) if pinned else None
+        self.host_status = ops.kernel_status_words() if pinned else None
         self.done = torch.cuda.Event() if pinned else None
         self.rows = 0
 
@@ -118,16 +118,6 @@ class Sampler:
         turn = self._turns[self._last if ticket is None else ticket]
         if turn.done is not None:
             turn.done.synchronize()
-        if turn.host_status is not None and any(turn.host_status.tolist()):
-            which = " and ".join(name for name, word in zip(("the few-rows product", "the tcgen05 prompt attention",
-                                                             "the attention over expanded latents", "the decode step",
-                                                             "the product on pairs of SMs", "the attention over 4-bit keys"),
-                                                            turn.host_status.tolist()) if word)
-            left_out = int(turn.host_status[2]) == ops.EXPANDED_ROWS_LEFT_OUT
-            turn.host_status.zero_()
-            ops.kernel_status_reset()
-            if left_out:
-                raise ops.KernelError("the attention over expanded latents was given room for fewer rows than the requests hold: "
-                                      "the step's results are not valid")
-            raise ops.KernelError(f"a bounded wait inside {which} gave up: the step's results are not valid")
+        if turn.host_status is not None:
+            ops.kernel_status_check(turn.host_status)
         return turn.host_out[:turn.rows].tolist()

@@ -61,3 +61,55 @@ def test_an_engine_of_small_pages_and_an_odd_number_of_them():
         made.append(engine.generate_many(prompts, GenerationConfig(max_new_tokens=9)))
         made[-1].append([beam.tokens for beams in engine.beam_search(prompts, 3, 6, 9) for beam in beams])
     assert made[0] == made[1]
+
+
+# ------------------------------------------------------------------ searches whose steps are not valid
+@pytest.mark.parametrize("count", [3, 24])
+def test_a_search_whose_kernels_gave_up_raises_and_leaves_the_engine_usable(count):
+    """The few-rows product is made to give up a wait (a test hook: a tile that never arrives and a small limit; the kernel
+    returns): beams of such steps are not handed out, and neither the pages nor the word are left to the next caller."""
+    from llm_serving_engine_b200 import GenerationConfig
+    from test_engine_gpu import engine_for, prompts_for
+    engine = engine_for("D", dtype="bfloat16", batch=6)
+    prompts = prompts_for("D", (9, 21), seed=4)
+    good, tokens = engine.beam_search(prompts, 3, count, 5), engine.generate_many(prompts, GenerationConfig(max_new_tokens=4))
+    ops.gemm_bf16_skinny_test_hooks(spin_limit=2000, withhold=True)
+    try:
+        with pytest.raises(ops.KernelError, match="bounded wait inside the few-rows product"):
+            engine.beam_search(prompts, 3, count, 5)
+    finally:
+        ops.gemm_bf16_skinny_test_hooks()
+    assert ops.gemm_bf16_skinny_status() == 0
+    assert not engine.cache.requests and engine.cache.groups[0].pool.used_pages == 0
+    assert engine.generate_many(prompts, GenerationConfig(max_new_tokens=4)) == tokens
+    assert engine.beam_search(prompts, 3, count, 5) == good
+
+
+@pytest.mark.parametrize("word", range(6))
+def test_every_status_word_fails_a_search(word, monkeypatch):
+    """Whichever kernel's word comes back set, at the look in between (16 tokens) or at the end."""
+    engine = engine_of(models(), kv_bits=4)
+    plain_read = ops.kernel_status_async
+
+    def spoilt(words):
+        plain_read(words)
+        torch.cuda.current_stream().synchronize()
+        words[word] = 1
+
+    for count in (4, 20):
+        monkeypatch.setattr(ops, "kernel_status_async", spoilt)
+        with pytest.raises(ops.KernelError, match=f"bounded wait inside {ops._STATUS_NAMES[word]}"):
+            engine.beam_search([[3, 5, 8]], 4, count, 9)
+        monkeypatch.setattr(ops, "kernel_status_async", plain_read)
+        assert not engine.cache.requests and len(engine.beam_search([[3, 5, 8]], 4, count, 9)[0]) == 4
+
+
+def test_logits_that_are_not_numbers_leave_no_beam_and_are_told():
+    model = models()
+    engine = engine_of(model)
+    kept = model.final_norm.weight.clone()
+    model.final_norm.weight.fill_(float("nan"))
+    with pytest.raises(ops.KernelError, match="not numbers"):
+        engine.beam_search([[3, 5, 8], [1]], 4, 5, 9)
+    model.final_norm.weight.copy_(kept)
+    assert not engine.cache.requests and [len(beams) for beams in engine.beam_search([[3, 5, 8], [1]], 4, 5, 9)] == [4, 4]
