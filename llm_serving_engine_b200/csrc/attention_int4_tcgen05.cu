@@ -1,14 +1,18 @@
 // Attention of prompt portions over keys and values held in 4 bits (int4_cache.cu), causal, on the 5th-generation tensor cores;
 // bfloat16 queries, head sizes 64 and 128, pages of any size.
 //
-// Two kernels (three when a launch has few blocks).
+// Three kernels (four when a launch has few blocks).
+//   measure   the largest magnitude of every tile of 128 keys, and of its values, that the scales and centres allow for.
 //   expand    the codes of every request's keys, page by page, become float16 values in a workspace: [head][row][D], a request's
 //             rows one after the other, rounded up to whole tiles of 128 with zeros.  Once for all query heads and row tiles that
 //             read them.  Float16 because a value s (u - 8) + c rounded to bfloat16 would be off by up to 2^-8, as much as the result's own
-//             rounding, and float16 by 2^-11; keys are scaled by 2^-8 and queries by 2^-4 (exact), which keeps scores of
-//             keys up to 2^24 in range.  A row that float16 does not hold, or that is not a number, becomes NaN in its key and
-//             zeros in its value: who attends to it gets NaN, and nobody else does.  The queries become float16 here as well (in
-//             attend every block's tensor cores waited 0.9 us for it).
+//             rounding, and float16 by 2^-11.  So that this holds for numbers of any size, a request's keys of a head, and its values, are
+//             multiplied by a power of two (exact) that takes the largest of them to 2^14 .. 2^15: a number down to 2^-28 of that is rounded
+//             by 2^-11 of itself, a smaller one by 2^-39 of the largest.  (With fixed powers, keys below 2^-6 and values below
+//             2^-14 lost their last bits.)  attend takes the powers back out of scores and results.  The queries become
+//             float16 here as well, each row of a head by a power of its own.  A row with a key beyond 2^24 or a
+//             value beyond 65,504, or that is not a number, becomes NaN in its key and zeros in its value: who attends to it gets
+//             NaN, and nobody else does.
 //   attend    one block = 128 score rows of one request and key/value head: (token, query head of the group) pairs, so that
 //             keys are brought in once for all heads of a group and portions of a few tokens fill the rows.  Keys are walked in tiles
 //             of 128, which go alternately to two groups of four softmax warps, each with its own key and value stage, accumulators in
@@ -16,8 +20,9 @@
 //               loader warp   TMA: the queries once, then a tile of keys or values per copy.
 //               MMA warps     one thread issues S = Q K^T (tcgen05.mma, tensor memory), one of another warp O += P V.
 //               softmax       a thread owns a row of its group's tiles: scores from tensor memory, maximum, exp2 in float32, float16
-//                             probabilities to shared memory in the layout that the tensor cores read.  O is rescaled
-//                             when a maximum has grown by more than 2^8 (at once beyond 2^14: float16 ends at 2^16).
+//                             probabilities (2^-11 of them; of those below 2^-14, 2^-25 of the largest) to shared memory in the
+//                             layout that the tensor cores read.  O is rescaled when a maximum has grown by more than 2^8 (at once
+//                             beyond 2^14: float16 ends at 2^16).
 //   combine   with fewer blocks than SMs, several blocks share the keys of a tile; each leaves its part in a workspace of this
 //             call, and another launch adds them up, in the order of the parts.
 // What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s (324 at the power cap): tensor
@@ -44,7 +49,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f, REDO_STEP = 14.0f;   // in powers of two
 constexpr int MIN_TILES_A_PART = 4, MAX_PARTS = 8;
 constexpr uint32_t HALF_BYTES = 128 * 128;                // 128 rows x 64 float16
-constexpr float KEY_SCALE = 1.0f / 256.0f, QUERY_SCALE = 1.0f / 16.0f, SCORE_SCALE = 4096.0f;
+constexpr float MOST_KEY = 65504.0f * 256.0f, MOST_VALUE = 65504.0f;       // rows beyond become NaN
 
 __device__ int lse_attn_int4_tc_error;
 
@@ -109,76 +114,141 @@ __device__ __forceinline__ void find_work(const int* segment_start, const int* f
   }
 }
 
+// The power of two that takes numbers of this biased exponent (of float32) to 2^14 .. 2^15, and its inverse.  2^74 at most, so that
+// the inverse times a weight stays a normal number: what is smaller than 2^-60 uses less of float16's range.
+__device__ __forceinline__ float unit_up(uint32_t exponent) { return __uint_as_float((268u - min(max(exponent, 67u), 254u)) << 23); }
+__device__ __forceinline__ float unit_down(uint32_t exponent) { return __uint_as_float((min(max(exponent, 67u), 254u) - 14u) << 23); }
+// The largest magnitude that a row's codes could stand for (not a number where the row is not one).
+__device__ __forceinline__ float most_of(float2 row) { return fabsf(row.y) + 8.f * fabsf(row.x); }
+
+// Whose tile of keys the tile-th of the workspace is, by a whole warp, 32 requests at a time: the request (-1: behind the last
+// request's tiles, -2: one that another kernel takes), its first key's number, the request's keys and its first tile.
+struct KeyTile { int seg, key0, keys, first; };
+__device__ __forceinline__ KeyTile find_keys(const int* segment_start, const int* first_pos, int num_segments, int skip_single, int tile) {
+  const int lane = threadIdx.x & 31;
+  KeyTile found = {-1, 0, 0, 0};
+  int before = 0;
+  for (int base = 0; base < num_segments && found.seg == -1; base += 32) {
+    const int s = base + lane;
+    int n = 0, ctx = 0, rows = 0;
+    if (s < num_segments) {
+      rows = segment_start[s + 1] - segment_start[s];
+      ctx = rows > 0 ? max(0, first_pos[s] + rows) : 0;
+      n = (ctx + BN - 1) / BN;
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned vote = __ballot_sync(0xffffffffu, n > 0 && tile >= before + incl - n && tile < before + incl);
+    if (vote) {
+      const int src = __ffs(vote) - 1;
+      found.first = before + __shfl_sync(0xffffffffu, incl - n, src);
+      found.key0 = (tile - found.first) * BN;
+      found.keys = __shfl_sync(0xffffffffu, ctx, src);
+      found.seg = __shfl_sync(0xffffffffu, skip_single && rows == 1 ? 1 : 0, src) ? -2 : base + src;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return found;
+}
+
+// ------------------------------------------------------------------ measure
+// One block = a tile and head: a thread a key's scale and centre, or its value's.
+__global__ void __launch_bounds__(2 * BN)
+measure_int4_kernel(const __nv_bfloat162* k_scales, const __nv_bfloat162* v_scales, uint2* __restrict__ tops,
+                    const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
+                    const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size, int num_pages, int skip_single) {
+  __shared__ KeyTile found_s;
+  __shared__ uint32_t top_s[2 * BN / 32];
+  pdl_launch_dependents();
+  const int tile = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+  if (tid < 32) {
+    const KeyTile found = find_keys(segment_start, first_pos, num_segments, skip_single, tile);
+    if (tid == 0) found_s = found;
+  }
+  __syncthreads();
+  const KeyTile at = found_s;
+  const int key = at.key0 + tid % BN;
+  const bool live = at.seg >= 0 && key < at.keys;
+  int page = 0;
+  const int logical = (unsigned)key / (unsigned)page_size;
+  if (live) page = LSE_CHECKED(block_tables[(size_t)at.seg * bt_stride + logical], 0, num_pages, 0, LSE_CHECK_TABLE_ENTRY);
+  pdl_wait();
+  float most = 0.f;
+  if (live) {
+    const size_t place = ((size_t)page * n_kv + head0 + head) * page_size + (key - logical * page_size);
+    most = most_of(__bfloat1622float2((tid < BN ? k_scales : v_scales)[place]));
+    if (!(most <= (tid < BN ? MOST_KEY : MOST_VALUE))) most = 0.f;       // (a row that becomes NaN)
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));      // (as whole numbers: none is negative)
+  if ((tid & 31) == 0) top_s[tid >> 5] = top;
+  __syncthreads();
+  if (tid == 0) {
+    uint2 tops_here = make_uint2(0, 0);
+    for (int w = 0; w < BN / 32; ++w) { tops_here.x = max(tops_here.x, top_s[w]); tops_here.y = max(tops_here.y, top_s[BN / 32 + w]); }
+    tops[(size_t)head * gridDim.x + tile] = tops_here;
+  }
+}
+
 // ------------------------------------------------------------------ expand
 // One block = EXPAND_KEYS keys of a tile and one head, keys and values; 256 threads, LANES = D / 8 of them a row, eight values each, all loads
 // of a thread on their way together (a block a tile, eight rows a thread one after the other: 17 us for 51 tiles of two heads).
 constexpr int EXPAND_KEYS = 32;
-constexpr int QUERY_PIECES = 4;      // 16 bytes each, of a thread of the blocks behind those (blockIdx.z), which make the queries float16
+// The blocks behind those (blockIdx.z) make the queries float16, QUERY_PIECES times 16 bytes a thread, a head's row by LANES neighbours.
+constexpr int QUERY_PIECES = 4;
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_int4_kernel(const unsigned char* k_codes, const __nv_bfloat162* k_scales,
                    const unsigned char* v_codes, const __nv_bfloat162* v_scales, uint4* __restrict__ k_out,
-                   uint4* __restrict__ v_out, const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
-                   const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size, int num_pages, int capacity,
-                   int skip_single, const uint4* q, uint4* q_out, long long q_pieces) {
+                   uint4* __restrict__ v_out, const uint2* tops, float2* units, const int* __restrict__ block_tables, int bt_stride,
+                   const int* __restrict__ segment_start, const int* __restrict__ first_pos, int num_segments, int n_kv, int head0, int page_size,
+                   int num_pages, int skip_single, const uint4* q, uint4* q_out, float* q_units, long long q_pieces) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES, MINE = EXPAND_KEYS / ROWS;      // rows at once, rows of a thread
-  __shared__ int found[3];
+  __shared__ KeyTile found_s;
   pdl_launch_dependents();
-  const int tile = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-  if (blockIdx.z >= BN / EXPAND_KEYS) {      // queries
+  const int tile = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, capacity = gridDim.x;
+  if (blockIdx.z >= BN / EXPAND_KEYS) {
     pdl_wait();
     const long long block = ((long long)(blockIdx.z - BN / EXPAND_KEYS) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
     uint4 w[QUERY_PIECES];
 #pragma unroll
     for (int k = 0; k < QUERY_PIECES; ++k) {
       const long long i = (block * QUERY_PIECES + k) * 256 + tid;
-      if (i < q_pieces) w[k] = q[i];
+      w[k] = i < q_pieces ? q[i] : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int k = 0; k < QUERY_PIECES; ++k) {
       const long long i = (block * QUERY_PIECES + k) * 256 + tid;
       uint32_t* x = &w[k].x;
+      uint32_t top = 0;       // the largest magnitude of the row, as the bits of a bfloat16
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, x[e] >> 16 & 0x7fffu));
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float up = unit_up(top >> 7);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]));
-        x[e] = pack_f16(v.x * QUERY_SCALE, v.y * QUERY_SCALE);
+        x[e] = pack_f16(v.x * up, v.y * up);
       }
-      if (i < q_pieces) q_out[i] = w[k];
+      if (i < q_pieces) {
+        q_out[i] = w[k];
+        if (i % LANES == 0) q_units[i / LANES] = unit_down(top >> 7);
+      }
     }
     return;
   }
-  // whose tile it is: the first warp walks the requests, 32 at a time
   if (tid < 32) {
-    int before = 0, seg = -1, at = 0, keys = 0;
-    for (int base = 0; base < num_segments && seg < 0; base += 32) {
-      const int s = base + lane;
-      int n = 0, ctx = 0, rows = 0;
-      if (s < num_segments) {
-        rows = segment_start[s + 1] - segment_start[s];
-        ctx = rows > 0 ? max(0, first_pos[s] + rows) : 0;
-        n = (ctx + BN - 1) / BN;
-      }
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const unsigned vote = __ballot_sync(0xffffffffu, n > 0 && tile >= before + incl - n && tile < before + incl);
-      if (vote) {
-        const int src = __ffs(vote) - 1;
-        at = tile - before - __shfl_sync(0xffffffffu, incl - n, src);
-        keys = __shfl_sync(0xffffffffu, ctx, src);
-        seg = __shfl_sync(0xffffffffu, skip_single && rows == 1 ? 1 : 0, src) ? -2 : base + src;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (lane == 0) { found[0] = seg; found[1] = at * BN; found[2] = keys; }
+    const KeyTile found = find_keys(segment_start, first_pos, num_segments, skip_single, tile);
+    if (tid == 0) found_s = found;
   }
   __syncthreads();
-  const int seg = found[0], key0 = found[1], keys = found[2];
+  const int seg = found_s.seg, key0 = found_s.key0, keys = found_s.keys, first = found_s.first;
   pdl_wait();                // (before any return: a launch without work must not end before the one before it)
-  if (seg < 0) return;       // behind the last request's tiles, or one that another kernel takes
+  if (seg < 0) return;
   const int c = tid % LANES, r0 = blockIdx.z * EXPAND_KEYS + tid / LANES;
   const size_t out0 = ((size_t)head * capacity + tile) * BN;
   const int* bt = block_tables + (size_t)seg * bt_stride;
@@ -199,13 +269,21 @@ expand_int4_kernel(const unsigned char* k_codes, const __nv_bfloat162* k_scales,
       vs[i] = v_scales[place];
     }
   }
+  // the largest of all the request's tiles, by every warp (the tiles that the workspace has no room for are not worked on)
+  uint2 top = make_uint2(0, 0);
+  for (int i = first + lane; i < min(capacity, first + (keys + BN - 1) / BN); i += 32) {
+    const uint2 t = tops[(size_t)head * capacity + i];
+    top.x = max(top.x, t.x); top.y = max(top.y, t.y);
+  }
+  const uint32_t k_exponent = __reduce_max_sync(0xffffffffu, top.x) >> 23, v_exponent = __reduce_max_sync(0xffffffffu, top.y) >> 23;
+  const float k_up = unit_up(k_exponent), v_up = unit_up(v_exponent);
+  if (tile == first && blockIdx.z == 0 && tid == 0) units[(size_t)head * capacity + tile] = make_float2(unit_down(k_exponent), unit_down(v_exponent));
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
-    float2 kf = __bfloat1622float2(ks[i]);
-    const float2 vf = __bfloat1622float2(vs[i]);
-    kf.x *= KEY_SCALE; kf.y *= KEY_SCALE;
-    // the largest magnitude that the row's codes could stand for; false for what is not a number
-    const bool fits = fabsf(kf.y) + 8.f * fabsf(kf.x) <= 65504.f && fabsf(vf.y) + 8.f * fabsf(vf.x) <= 65504.f;
+    float2 kf = __bfloat1622float2(ks[i]), vf = __bfloat1622float2(vs[i]);
+    const bool fits = most_of(kf) <= MOST_KEY && most_of(vf) <= MOST_VALUE;      // false for what is not a number
+    kf.x *= k_up; kf.y *= k_up;
+    vf.x *= v_up; vf.y *= v_up;
     auto values = [](uint32_t x, float2 s) {
       uint32_t w[4];
 #pragma unroll
@@ -227,7 +305,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out, const int* __restrict__ segment_start,
                    const int* __restrict__ first_pos, int num_segments, int n_q, int group, int heads, int head0, int tokens_a_tile,
-                   float scale_log2e, int capacity, int skip_single, int parts, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+                   float scale_log2e, int capacity, int skip_single, int parts, const float2* units, const float* q_units,
+                   float* __restrict__ part_o, float2* __restrict__ part_ml) {
   constexpr int HALVES = D / 64;
   constexpr uint32_t Q_BYTES = HALVES * HALF_BYTES, KV_BYTES = HALVES * HALF_BYTES, P_BYTES = 2 * HALF_BYTES;
   constexpr uint32_t GROUP_BYTES = HALVES * 1024;          // 8 keys in a stage
@@ -353,6 +432,12 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t s_addr = lane_addr + g * S_COLS, o_addr = lane_addr + O_COL + g * D;
     const int my_pos = pos0 + min(row, nrows - 1) / group;
     unsigned char* prow = gbase + (p_s - base) + g * P_BYTES + row * 128;
+    // the powers of two in this row's scores and in the values
+    const float2 unit = units[(size_t)head * capacity + tile0];
+    const int my_row = min(row, nrows - 1);
+    const double exact_scale = (double)scale_log2e * (double)q_units[(long long)(row_base + my_row / group) * n_q + (head0 + head) * group + my_row % group] * (double)unit.x;
+    const float row_scale = (float)fmin(fmax(exact_scale, 0x1p-126), 0x1p127);      // (beyond, scores are all alike, or infinitely far apart)
+    const uint64_t scale_pair = f32_pair(row_scale, row_scale);      // (made here: 340 us for the 2,048 rows below; in the loop 347)
     float m_used = -INFINITY, m_seen = -INFINITY, l = 0.f;   // the maximum that O and l are relative to; the largest score seen
     bool pending = false;                                    // m_seen has outgrown m_used: O and l are to be rescaled
     bool ok = true;                                          // the same in all lanes of a warp (a vote after every wait)
@@ -386,7 +471,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
         for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])));
       }
-      const float m_tile = mx * scale_log2e;
+      const float m_tile = mx * row_scale;
       if (j < GROUPS) {
         m_used = m_seen = m_tile;
       } else {
@@ -417,7 +502,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         tmem_st_wait();
       }
       const float neg = m_used == -INFINITY ? 0.f : -m_used;
-      const uint64_t scale_pair = f32_pair(scale_log2e, scale_log2e), neg_pair = f32_pair(neg, neg);
+      const uint64_t neg_pair = f32_pair(neg, neg);
       uint64_t sum_pair = 0;
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {
@@ -458,7 +543,7 @@ attend_int4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const float w_other = m_other == -INFINITY ? (l_other == 0.f ? 0.f : 1.f) : exp2_fast(m_other - m_all);
     const float l_all = g == 0 ? fmaf(l_other, w_other, l * w_mine) : fmaf(l, w_mine, l_other * w_other);
     const bool shared = sharing > 1;
-    const float inv = shared ? 1.0f : 1.0f / l_all;
+    const float inv = shared ? unit.y : unit.y / l_all;
     const float w0 = (g == 0 ? w_mine : w_other) * inv, w1 = (g == 0 ? w_other : w_mine) * inv;
     const int n0 = (n_local + 1) / 2, n1 = n_local / 2;     // tiles of the groups
     if (ok) ok = wait_all(B_OD + 0, (uint32_t)(n0 - 1) & 1u);
@@ -590,7 +675,7 @@ template <int D>
 int launch_portions(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* out,
                     const int* block_tables, int bt_stride, const int* segment_start, const int* first_pos, int num_segments, int tokens,
                     long long num_pages, int n_q, int n_kv, int page_size, float scale, int skip_single, int with_tiles, int capacity,
-                    int heads_at_once, int parts, void* keys, void* values, void* queries, float* scratch, cudaStream_t stream) {
+                    int heads_at_once, int parts, void* keys, void* values, void* queries, void* powers, float* scratch, cudaStream_t stream) {
   static SmemAllowance allowance;
   const size_t smem = attend_smem<D>();
   cudaError_t err = allow_smem(attend_int4_kernel<D>, smem, allowance);
@@ -599,6 +684,9 @@ int launch_portions(const void* q, const void* k_codes, const void* k_scales, co
   const int tiles = (tokens + tokens_a_tile - 1) / tokens_a_tile + with_tiles;
   float* part_o = parts > 1 ? scratch : nullptr;
   float2* part_ml = parts > 1 ? reinterpret_cast<float2*>(scratch + (size_t)tokens * n_q * parts * D) : nullptr;
+  float2* units = reinterpret_cast<float2*>(powers);
+  uint2* tops = reinterpret_cast<uint2*>(units + (size_t)heads_at_once * capacity);
+  float* q_units = reinterpret_cast<float*>(tops + (size_t)heads_at_once * capacity);
   CUtensorMap map_q, map_k, map_v;
   for (int head0 = 0; head0 < n_kv; head0 += heads_at_once) {
     const int heads = n_kv - head0 < heads_at_once ? n_kv - head0 : heads_at_once;
@@ -608,14 +696,18 @@ int launch_portions(const void* q, const void* k_codes, const void* k_scales, co
       return LSE_ERR_BAD_ARGUMENT;
     const long long q_pieces = head0 == 0 ? (long long)tokens * n_q * (D / 8) : 0, a_layer = (long long)capacity * heads * 256 * QUERY_PIECES;
     if (q_pieces / a_layer > 60000) return LSE_ERR_TOO_LARGE;
-    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads, (unsigned)(BN / EXPAND_KEYS + (q_pieces + a_layer - 1) / a_layer)), dim3(256), 0, stream, (const unsigned char*)k_codes,
-                     (const __nv_bfloat162*)k_scales, (const unsigned char*)v_codes, (const __nv_bfloat162*)v_scales, (uint4*)keys,
-                     (uint4*)values, block_tables, bt_stride, segment_start, first_pos, num_segments, n_kv, head0, page_size,
-                     (int)num_pages, capacity, skip_single, (const uint4*)q, (uint4*)queries, q_pieces);
+    err = lse_launch(measure_int4_kernel, dim3((unsigned)capacity, (unsigned)heads), dim3(2 * BN), 0, stream,
+                     (const __nv_bfloat162*)k_scales, (const __nv_bfloat162*)v_scales, tops, block_tables, bt_stride, segment_start,
+                     first_pos, num_segments, n_kv, head0, page_size, (int)num_pages, skip_single);
+    if (err != cudaSuccess) return (int)err;
+    err = lse_launch(expand_int4_kernel<D>, dim3((unsigned)capacity, (unsigned)heads, (unsigned)(BN / EXPAND_KEYS + (q_pieces + a_layer - 1) / a_layer)), dim3(256), 0,
+                     stream, (const unsigned char*)k_codes, (const __nv_bfloat162*)k_scales, (const unsigned char*)v_codes, (const __nv_bfloat162*)v_scales,
+                     (uint4*)keys, (uint4*)values, (const uint2*)tops, units, block_tables, bt_stride, segment_start, first_pos, num_segments, n_kv,
+                     head0, page_size, (int)num_pages, skip_single, (const uint4*)q, (uint4*)queries, q_units, q_pieces);
     if (err != cudaSuccess) return (int)err;
     err = lse_launch(attend_int4_kernel<D>, dim3((unsigned)((long long)tiles * heads * parts)), dim3(THREADS), smem, stream, map_q, map_k,
                      map_v, (__nv_bfloat16*)out, segment_start, first_pos, num_segments, n_q, group, heads, head0, tokens_a_tile,
-                     scale * LOG2E * SCORE_SCALE, capacity, skip_single, parts, part_o, part_ml);
+                     scale * LOG2E, capacity, skip_single, parts, (const float2*)units, (const float*)q_units, part_o, part_ml);
     if (err != cudaSuccess) return (int)err;
     if (parts > 1) {
       err = lse_launch(combine_tiles_kernel<D>, dim3((unsigned)(tiles * heads), BM / 8), dim3(256), 0, stream, (const float*)part_o,
@@ -645,23 +737,24 @@ extern "C" int lse_attention_int4_tc_status_reset(void) {
 // q, out bfloat16 [tokens, n_q, head_dim]; the cache as int4_cache.cu leaves it; segment_start [S + 1]: first row of each request's
 // portion, first_pos [S]: that row's position.  keys, values: float16 [heads_at_once, capacity * 128, head_dim], capacity = tiles of 128
 // keys of all requests together, each request's rounded up (rows of a request that does not fit come out as NaN).  with_tiles: requests
-// that have rows here, at most.  queries: float16 [tokens, n_q, head_dim].  parts > 1 (at most 8): scratch holds tokens * n_q * parts * (head_dim + 2) float32.
+// that have rows here, at most.  queries: float16 [tokens, n_q, head_dim].  powers: 4 heads_at_once capacity + tokens n_q words.  parts > 1
+// (at most 8): scratch holds tokens * n_q * parts * (head_dim + 2) float32.
 extern "C" int lse_paged_attention_prefill_int4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                                                 const void* v_scales, void* out, const int* block_tables, int bt_stride,
                                                 const int* segment_start, const int* first_pos, int num_segments, int tokens,
                                                 long long num_pages, int n_q, int n_kv, int head_dim, int page_size, float scale,
                                                 int skip_single, int with_tiles, int capacity, int heads_at_once, int parts, void* keys,
-                                                void* values, void* queries, float* scratch, cudaStream_t stream) {
+                                                void* values, void* queries, void* powers, float* scratch, cudaStream_t stream) {
   if (tokens <= 0 || num_segments <= 0) return 0;
   if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_q % n_kv || n_q / n_kv > BM || page_size <= 0 || num_pages <= 0 ||
       num_pages * page_size > 0x7fffffffLL || !(scale > 0.f) || capacity < 1 || heads_at_once < 1 || parts < 1 || parts > MAX_PARTS ||
-      with_tiles < 1 || keys == nullptr || values == nullptr || queries == nullptr || (parts > 1 && scratch == nullptr) ||
+      with_tiles < 1 || keys == nullptr || values == nullptr || queries == nullptr || powers == nullptr || (parts > 1 && scratch == nullptr) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)keys | (uintptr_t)values |
-        (uintptr_t)queries | (uintptr_t)scratch) & 15) || (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3))
+        (uintptr_t)queries | (uintptr_t)powers | (uintptr_t)scratch) & 15) || (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3))
     return LSE_ERR_BAD_ARGUMENT;
   if (heads_at_once > 65535 || (long long)heads_at_once * capacity * (BN / 8) > 0x7fffffffLL) return LSE_ERR_TOO_LARGE;
 #define LSE_INT4_ARGS q, k_codes, k_scales, v_codes, v_scales, out, block_tables, bt_stride, segment_start, first_pos, num_segments, \
-  tokens, num_pages, n_q, n_kv, page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts, keys, values, queries, scratch, stream
+  tokens, num_pages, n_q, n_kv, page_size, scale, skip_single, with_tiles, capacity, heads_at_once, parts, keys, values, queries, powers, scratch, stream
   return head_dim == 128 ? launch_portions<128>(LSE_INT4_ARGS) : launch_portions<64>(LSE_INT4_ARGS);
 #undef LSE_INT4_ARGS
 }

@@ -26,7 +26,7 @@ _SIGNATURES = {
                                         c_longlong, c_int, c_void_p],
     "lse_paged_attention_prefill_int4": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                          c_void_p, c_int, c_int, c_longlong, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
-                                         c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+                                         c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "lse_beam_select_scratch_kb": [c_int, c_int, c_int],
     "lse_beam_select": [c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                         c_void_p, c_void_p, c_void_p],

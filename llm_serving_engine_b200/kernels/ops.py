@@ -2317,7 +2317,7 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     q, out bfloat16 [T, n_q, D], D 64 or 128, at most 128 query heads a key/value head; segment_start int32 [S + 1],
     segment_first_position int32 [S].  ``keys``: keys that the requests hold together, at most (0: what the block tables have room
     for); keys and values are worked on as float16 in a workspace of that size (a request beyond it comes out as NaN, as do rows
-    that attend to a value that float16 does not hold: 65,504; keys: 2^24).  ``skip_single``: requests of one row are left to
+    that attend to a value beyond 65,504 or a key beyond 2^24; small numbers keep float16's 11 bits: see the kernel).  ``skip_single``: requests of one row are left to
     :func:`paged_attention_decode_int4`; ``max_portions`` (with it): at most so many requests have more."""
     name = "paged_attention_prefill_int4"
     pages, n_kv, page_size, dim = _int4_pages(name, k_codes, k_scales, v_codes, v_scales)
@@ -2345,17 +2345,19 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     # several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs
     blocks = (-(-tokens // (INT4_TILE // group)) + with_tiles) * heads_at_once
     parts = max(1, min(8, 5 * sm_count() // (4 * blocks)))
-    # float16 keys, values and queries, and (several parts) float32 outputs, maxima and sums of every part
+    # float16 keys, values and queries, the powers of two in them, and (several parts) float32 outputs, maxima and sums of every part
     halves = heads_at_once * a_head
     queries = tokens * n_q * dim
-    workspace = torch.empty(4 * halves + 2 * queries + (4 * tokens * n_q * parts * (dim + 2) if parts > 1 else 0), dtype=_U8, device=q.device)
+    powers = 4 * halves + 2 * queries
+    parts_at = powers + 16 * heads_at_once * capacity + (4 * tokens * n_q + 15) // 16 * 16
+    workspace = torch.empty(parts_at + (4 * tokens * n_q * parts * (dim + 2) if parts > 1 else 0), dtype=_U8, device=q.device)
     at = workspace.data_ptr()
     check(library.load().lse_paged_attention_prefill_int4(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                                                           v_scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), table_stride,
                                                           segment_start.data_ptr(), segment_first_position.data_ptr(), segments,
                                                           tokens, pages, n_q, n_kv, dim, page_size, scale, skip_single, with_tiles,
-                                                          capacity, heads_at_once, parts, at, at + 2 * halves, at + 4 * halves,
-                                                          at + 4 * halves + 2 * queries if parts > 1 else None, _current_stream(device)), name)
+                                                          capacity, heads_at_once, parts, at, at + 2 * halves, at + 4 * halves, at + powers,
+                                                          at + parts_at if parts > 1 else None, _current_stream(device)), name)
     return out
 
 

@@ -113,3 +113,53 @@ def test_logits_that_are_not_numbers_leave_no_beam_and_are_told():
         engine.beam_search([[3, 5, 8], [1]], 4, 5, 9)
     model.final_norm.weight.copy_(kept)
     assert not engine.cache.requests and [len(beams) for beams in engine.beam_search([[3, 5, 8], [1]], 4, 5, 9)] == [4, 4]
+
+
+# ------------------------------------------------------------------ prompt portions over numbers of any size
+def times(cache, keys, values):
+    """The cache of ``keys`` times its keys and ``values`` times its values (powers of two: scales and centres hold them exactly)."""
+    return cache[0], (cache[1].float() * keys).bfloat16(), cache[2], (cache[3].float() * values).bfloat16()
+
+
+@pytest.mark.parametrize("counts,firsts,n_q,n_kv,dim", [([130, 1, 9], [20, 5, 700], 6, 2, 64), ([70], [3000], 5, 1, 128)])
+@pytest.mark.parametrize("key,query,value", [(-14, 0, -14), (-28, 6, -28), (-10, -20, -40), (6, 100, -5), (-50, 50, 8), (0, -60, 3)])
+def test_portions_know_no_size(counts, firsts, n_q, n_kv, dim, key, query, value):
+    """Keys, queries and values times powers of two, the score's scale divided by them: the same results, to the last bit, times the values'.
+    (Every rounding is relative: nothing is small enough to lose bits, and nothing large enough to leave the range.)"""
+    g, cache, tables, start, first = portion_case(counts, firsts, n_kv, dim, 16, 11)
+    q = torch.randn((sum(counts), n_q, dim), generator=g).bfloat16().cuda()
+    want = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.125)
+    assert portions(cache, tables, counts, firsts, q, want, 0.125, 16) >= 8
+    got = ops.paged_attention_prefill_int4((q.float() * 2.0 ** query).bfloat16(), *times(cache, 2.0 ** key, 2.0 ** value), torch.empty_like(q), tables, start, first,
+                                           0.125 * 2.0 ** (-key - query))
+    assert torch.isfinite(want.float()).all() and torch.equal(got, (want.float() * 2.0 ** value).bfloat16())
+
+
+@pytest.mark.parametrize("page_size", [16, 5])
+def test_portions_whose_requests_and_heads_are_of_different_sizes(page_size):
+    """A request's numbers do not decide about another's bits, nor a head's about another's; within a request, keys and values that
+    grow by 2^20 from its first to its last, so that early rows see small ones only."""
+    counts, firsts, n_kv, dim = [40, 150, 33], [0, 200, 600], 2, 64
+    g, cache, tables, start, first = portion_case(counts, firsts, n_kv, dim, page_size, 12)
+    q = torch.randn((sum(counts), 6, dim), generator=g).bfloat16().cuda()
+    for s, (size, steepness) in enumerate(((-20, 0), (2, 0), (-12, 20))):
+        pages = tables[s][tables[s] >= 0].long()
+        ramp = 2.0 ** (size + torch.linspace(-steepness, 0, len(pages)).round().cuda()).view(-1, 1, 1, 1)
+        heads = torch.tensor([1.0, 2.0 ** -9], device="cuda").view(1, 2, 1, 1)
+        for scales in (cache[1], cache[3]):
+            scales[pages] = (scales[pages].float() * ramp * heads).bfloat16()
+    q[:40] *= 2.0 ** 18
+    out = ops.paged_attention_prefill_int4(q, *cache, torch.empty_like(q), tables, start, first, 0.5)
+    assert portions(cache, tables, counts, firsts, q, out, 0.5, page_size) >= 15
+
+
+def test_portions_over_zeros():
+    """Keys that are all zero weigh alike; values that are all zero give zeros."""
+    counts, firsts = [40], [100]
+    g, cache, tables, start, first = portion_case(counts, firsts, 1, 64, 16, 13)
+    q = torch.randn((40, 2, 64), generator=g).bfloat16().cuda()
+    for keys, values in ((0.0, 1.0), (1.0, 0.0), (0.0, 0.0)):
+        some = times(tuple(t.nan_to_num(0.0) if t.is_floating_point() else t for t in cache), keys, values)
+        out = ops.paged_attention_prefill_int4(q, *some, torch.empty_like(q), tables, start, first, 0.125)
+        assert portions(some, tables, counts, firsts, q, out, 0.125, 16) >= 6
+        assert values or not out.any()
