@@ -15,8 +15,8 @@
 // launches' latencies.  Pieces of twice the length 37 to 40 us, one more block an SM 38, loads past the L1 44.
 //
 // The last kernels of a step: the next step's read its block tables before they wait for the kernels before them (scores, tokens and parents
-// after that).  So merge and reorder never let the next kernel start early, and reorder's threads end only when the tables that they
-// wrote are visible to the whole device.
+// after that).  So merge and reorder never let the next kernel start early, reorder's threads that write tables end with a fence, and the
+// engine's beam search has ordinary launches between them and the step.
 #include "common.cuh"
 
 namespace {

@@ -5,8 +5,9 @@
 // Request s brings counts[s] tokens behind first[s] earlier ones and owns pages[page_start[s] .. page_start[s + 1]).  Every block
 // of the rows adds up all counts itself, 256 at a time (a step holds hundreds of requests at most), and looks its rows up in the
 // running sums, so one launch does it: what bounds it is the launch and two dependent loads, not the few hundred KB written.
-// The step's kernels read this metadata before they wait for the kernels before them, so this one never lets the next start early, and
-// its threads end only when what they wrote is visible to the whole device.
+// The step's kernels read this metadata before they wait for the kernels before them.  So this one never lets the next start early, its
+// threads end with a fence, and the beam search puts an ordinary launch between it and the step (visibility is promised behind a
+// wait or a complete launch, not behind a fence).
 #include "common.cuh"
 
 namespace {

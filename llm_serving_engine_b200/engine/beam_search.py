@@ -215,8 +215,10 @@ class _Step:
             ops.step_tables(held.row_lengths, held.ones, pages, held.page_start, cache.page_size, step.segment_start,
                             step.segment_of_token, step.positions, held.maps[index] if held.maps else torch.empty_like(step.positions),
                             step.segment_context, held.spare_tables)
-        logits = held.runner.model.forward(step, held.caches)
+        # An ordinary launch between the tables and the step: the step's first kernels may start before the launch behind which they are
+        # queued has ended and read the step's metadata at once, so the tables have to be complete and visible before that launch begins.
         held.lengths += 1
+        logits = held.runner.model.forward(step, held.caches)
         held.row_lengths += 1
         return logits
 

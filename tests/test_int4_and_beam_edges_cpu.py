@@ -22,3 +22,40 @@ def test_tables_whose_rows_overlap_are_not_written(tables):
         ops.beam_reorder(ints(1, 3), tables, ints(1), ints(3, 4), 16, [])
     with pytest.raises(KernelError, match="CUDA tensors only"):
         ops.step_tables(ints(1), ints(1), ints(9), ints(2), 16, ints(2), ints(5), ints(5), ints(5), ints(1), tables[:1])
+
+
+def test_an_ordinary_launch_lies_between_a_steps_tables_and_its_kernels(monkeypatch):
+    """The step's kernels may read tables, positions and slots before their wait for the launch before them: that launch is none of those
+    that write these."""
+    from types import SimpleNamespace
+
+    from llm_serving_engine_b200.engine import beam_search
+
+    order = []
+
+    class Counted:
+        def __init__(self, name):
+            self.name = name
+
+        def __iadd__(self, one):
+            order.append(self.name)
+            return self
+
+        def copy_(self, other):
+            order.append(self.name)
+
+        def view(self, *shape):
+            return self
+
+    monkeypatch.setattr(beam_search.ops, "beam_reorder", lambda *a: order.append("reorder"))
+    monkeypatch.setattr(beam_search.ops, "step_tables", lambda *a: order.append("tables"))
+    for states in ([], ["state"]):
+        order.clear()
+        runner = SimpleNamespace(cache=SimpleNamespace(page_size=16), model=SimpleNamespace(forward=lambda *a: order.append("step")))
+        step = SimpleNamespace(segment_start=None, segment_of_token=None, positions=None, segment_context=None)
+        held = SimpleNamespace(runner=runner, step=step, states=states, tables=[Counted("own tables")] * 2, new_tables=[None] * 2, storages=[[]] * 2,
+                               parents=None, lengths=Counted("lengths"), row_lengths=Counted("row lengths"), one=None, ones=None, slots=Counted("slots"),
+                               new_slots=None, page_start=None, maps=[None] * 2, spare_tables=None, caches=None)
+        beam_search._Step(held, 0, False)._launch()
+        at = order.index("step")
+        assert {"own tables", "tables"} <= set(order[:at]) and order[at - 1] == "lengths" and "row lengths" in order[at:]
