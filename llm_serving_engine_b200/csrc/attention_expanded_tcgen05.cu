@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x
 
 // rows[r] for r < capacity: a warp a row; rows of no request, and those that round a request up, are zeros.
 __global__ void __launch_bounds__(256)
-latent_gather_kernel(const __nv_bfloat16* __restrict__ cache, const int* __restrict__ block_tables, int bt_stride,
+latent_gather_kernel(const __nv_bfloat16* cache, const int* __restrict__ block_tables, int bt_stride,
                      const int* __restrict__ first, const int* __restrict__ context, int num_segments, int width,
                      int page_size, int num_pages, int window, __nv_bfloat16* __restrict__ rows, int capacity) {
   pdl_launch_dependents();
@@ -146,7 +146,7 @@ attn_expanded_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         __nv_bfloat16* __restrict__ out, const int* __restrict__ segment_start, const int* __restrict__ first,
                         const int* __restrict__ context, int num_segments, int heads, int first_head, int own_heads, int rank,
                         float scale_log2e, int window,
-                        const float* __restrict__ sink, const float* __restrict__ out_gate) {
+                        const float* __restrict__ sink, const float* out_gate) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gbase = smem_raw + (base - smem_u32(smem_raw));

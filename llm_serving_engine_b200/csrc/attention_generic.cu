@@ -66,7 +66,7 @@ __device__ __forceinline__ void chunk_softmax(float (&s)[2], float& m, float& l)
 // the divisions by the page size stood before every sixteen bytes (35 us a chunk of a tile against 12).
 // VEC: sixteen bytes at a time.
 template <typename T, bool VEC>
-__device__ __forceinline__ void fill_rows(float* dst, int pitch, const T* __restrict__ src, int rows, int D,
+__device__ __forceinline__ void fill_rows(float* dst, int pitch, const T* src, int rows, int D,
                                           const long long* offsets) {
   constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
   const int pieces = D / N;
@@ -155,7 +155,7 @@ __device__ __forceinline__ long long key_offset(const Step& p, const int* bt, in
 // near the time that the chunk's bytes take.
 template <typename T, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
-paged_attention_generic_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
+paged_attention_generic_kernel(const T* q, const T* k_cache, const T* v_cache,
                                T* __restrict__ out, const Step p, float* __restrict__ partials, int rows) {
   extern __shared__ __align__(16) float smem[];
   pdl_launch_dependents();
@@ -307,7 +307,7 @@ paged_attention_generic_kernel(const T* __restrict__ q, const T* __restrict__ k_
 // for two blocks an SM (102 KB each at 128 values): one loads while the other multiplies.
 template <typename T, int DT, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(THREADS, SPLIT && DT <= 64 ? 4 : 2)
-paged_attention_tiles_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
+paged_attention_tiles_kernel(const T* q, const T* k_cache, const T* v_cache,
                              T* __restrict__ out, const Step p, const int* __restrict__ segment_first,
                              float* __restrict__ partials, int tiles) {
   constexpr int TN = DT / 16;                 // columns of a thread: 4 (up to 64 values) or 8, in groups of four
@@ -535,7 +535,7 @@ paged_attention_tiles_kernel(const T* __restrict__ q, const T* __restrict__ k_ca
 constexpr int MERGE_BATCH = 32;
 template <typename T>
 __global__ void __launch_bounds__(MAX_D)
-paged_attention_generic_merge_kernel(const float* __restrict__ partials, T* __restrict__ out, const Step p) {
+paged_attention_generic_merge_kernel(const float* partials, T* __restrict__ out, const Step p) {
   __shared__ float wa_s[MERGE_BATCH], wb_s[MERGE_BATCH], sum_s[MERGE_BATCH];
   pdl_launch_dependents();
   const int index = blockIdx.x, head = blockIdx.y, d = threadIdx.x;

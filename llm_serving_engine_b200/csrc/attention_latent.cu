@@ -44,7 +44,7 @@ constexpr int PREP_THREADS = 128;
 // reads it there; else (a row too wide for that) every pass adds them up again from global memory.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(PREP_THREADS)
-latent_prepare_kernel(const TI* __restrict__ proj, int n_partials, long long partial_stride, long long ld,
+latent_prepare_kernel(const TI* proj, int n_partials, long long partial_stride, long long ld,
                       int q_off, int q_rank, const float* __restrict__ q_norm, TO* __restrict__ q_latent,
                       int kv_off, int rank, const float* __restrict__ kv_norm, int rot, int rot_dims,
                       const double* __restrict__ freq, float rot_factor, const int* __restrict__ positions,
@@ -120,7 +120,7 @@ latent_prepare_kernel(const TI* __restrict__ proj, int n_partials, long long par
 // q_plain [T][heads][dim] gets the unrotated part, q_wide [T][heads][wide] gets the rotated part at column `at`.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(128)
-latent_query_kernel(const TI* __restrict__ proj, int n_partials, long long partial_stride, long long ld, int q_off,
+latent_query_kernel(const TI* proj, int n_partials, long long partial_stride, long long ld, int q_off,
                     int heads, int dim, int rot, int rot_dims, const double* __restrict__ freq, float rot_factor,
                     const int* __restrict__ positions, const int* __restrict__ segment_of_token,
                     TO* __restrict__ q_plain, TO* __restrict__ q_wide, int wide, int at) {
@@ -155,7 +155,7 @@ latent_query_kernel(const TI* __restrict__ proj, int n_partials, long long parti
 constexpr int GATES_A_BLOCK = 512;
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(PREP_THREADS)
-latent_front_kernel(const TI* __restrict__ proj, int n_partials, long long partial_stride, long long ld, int q_off, int heads,
+latent_front_kernel(const TI* proj, int n_partials, long long partial_stride, long long ld, int q_off, int heads,
                     int dim, int rot, int rot_dims, const double* __restrict__ freq, float rot_factor, int kv_off, int rank,
                     const float* __restrict__ kv_norm, float eps, const int* __restrict__ positions,
                     const int* __restrict__ slot_mapping, TO* __restrict__ q_plain, TO* __restrict__ q_wide, int wide,
@@ -232,7 +232,7 @@ __device__ __forceinline__ uint4 lat_turn8(const uint4& raw, const float* cs, co
 }
 
 __global__ void __launch_bounds__(ROWS_THREADS)
-latent_front_rows_kernel(const __nv_bfloat16* __restrict__ proj, long long ld, int q_off, int heads, int dim, int rot, int rot_dims,
+latent_front_rows_kernel(const __nv_bfloat16* proj, long long ld, int q_off, int heads, int dim, int rot, int rot_dims,
                          const double* __restrict__ freq, float rot_factor, int kv_off, int rank, const float* __restrict__ kv_norm,
                          float eps, const int* __restrict__ positions, const int* __restrict__ slot_mapping,
                          __nv_bfloat16* __restrict__ q_plain, __nv_bfloat16* __restrict__ q_wide, int wide,
@@ -315,7 +315,7 @@ __device__ __forceinline__ float merge_sink(float& M, float& L, float sink) {
 // [t][head][chunk][DV + 2].
 template <typename T, int DPT, bool SPLIT>
 __global__ void __launch_bounds__(THREADS)
-latent_attention_kernel(const T* __restrict__ q, const T* __restrict__ cache, T* __restrict__ out,
+latent_attention_kernel(const T* q, const T* cache, T* __restrict__ out,
                         const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_of_token,
                         const int* __restrict__ positions, const float* __restrict__ sink, int n_q, int DK, int DV,
                         int page_size, float scale, int window, int num_pages, int num_segments,
@@ -472,7 +472,7 @@ latent_attention_kernel(const T* __restrict__ q, const T* __restrict__ cache, T*
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-latent_attention_merge_kernel(const float* __restrict__ partials, T* __restrict__ out,
+latent_attention_merge_kernel(const float* partials, T* __restrict__ out,
                               const int* __restrict__ segment_of_token, const int* __restrict__ positions,
                               const float* __restrict__ sink, int n_q, int DV, int window, int max_chunks,
                               int num_segments, int chunk_keys) {

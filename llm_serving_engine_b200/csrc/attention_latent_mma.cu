@@ -64,7 +64,7 @@ struct Layout {
 // NT: tiles of 8 output columns a warp owns (8 warps * NT * 8 >= DV).
 template <int NT>
 __global__ void __launch_bounds__(THREADS, 1)
-latent_attention_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ cache,
+latent_attention_mma_kernel(const __nv_bfloat16* q, const __nv_bfloat16* cache,
                             __nv_bfloat16* __restrict__ out, const int* __restrict__ block_tables, int bt_stride,
                             const int* __restrict__ segment_start, const int* __restrict__ segment_first_position,
                             const float* __restrict__ sink, int num_segments, int n_q, int DK, int DV, int page_size,

@@ -81,8 +81,8 @@ constexpr int BT_STAGE = 1024;   // block-table entries a block keeps in shared 
 // themselves up through distributed shared memory; else through global partial sums and a counter.
 template <int D, bool CLUSTER>
 __global__ void __launch_bounds__(128)
-attn_decode_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ kc,
-                   const __nv_bfloat16* __restrict__ vc, __nv_bfloat16* __restrict__ out,
+attn_decode_kernel(const __nv_bfloat16* q, const __nv_bfloat16* kc,
+                   const __nv_bfloat16* vc, __nv_bfloat16* __restrict__ out,
                    float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ arrivals,
                    const int* __restrict__ block_tables, int bt_stride,
                    const int* __restrict__ segment_of_token, const int* __restrict__ positions,
@@ -457,8 +457,8 @@ constexpr int PF_BN = 64;   // keys per tile
 
 template <int D>
 __global__ void __launch_bounds__(128)
-attn_prefill_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ kc,
-                    const __nv_bfloat16* __restrict__ vc, __nv_bfloat16* __restrict__ out,
+attn_prefill_kernel(const __nv_bfloat16* q, const __nv_bfloat16* kc,
+                    const __nv_bfloat16* vc, __nv_bfloat16* __restrict__ out,
                     const int* __restrict__ block_tables, int bt_stride,
                     const int* __restrict__ segment_start, const int* __restrict__ segment_first_pos,
                     int num_segments, int n_q, int n_kv, int page_size, float scale_log2e,

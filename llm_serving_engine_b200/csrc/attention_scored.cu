@@ -63,13 +63,13 @@ __device__ __forceinline__ float add_sink(float M, float& L, float sink) {
 // Output element of (row t, head h, value slot c, column d): ((t * n_q + h) * n_values + c) * dv + d.
 template <typename T, typename TO, bool SPLIT>
 __global__ void __launch_bounds__(THREADS)
-attention_scored_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
+attention_scored_kernel(const T* q, const T* k_cache, const T* v_cache,
                         TO* __restrict__ out, const int* __restrict__ block_tables, int bt_stride,
                         const int* __restrict__ segment_of_token, const int* __restrict__ positions,
-                        const float* __restrict__ r1, const float* __restrict__ r2, const float* __restrict__ sink,
+                        const float* r1, const float* r2, const float* __restrict__ sink,
                         int n_q, int n_kv, int dk, int dv, int n_values, int page_size, float scale, int num_pages,
                         int num_segments, float* __restrict__ partials, int max_chunks, int window, int keep_first, float cap,
-                        const float* __restrict__ head_bias, const float* __restrict__ out_gate) {
+                        const float* __restrict__ head_bias, const float* out_gate) {
   extern __shared__ float smem[];
   pdl_launch_dependents();
   pdl_wait();
@@ -271,10 +271,10 @@ attention_scored_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, 
 // The chunks of a row, head and value slot, left by the SPLIT kernel, merged in order: grid (tokens, n_q * n_values).
 template <typename TO>
 __global__ void __launch_bounds__(MAX_D)
-attention_scored_merge_kernel(const float* __restrict__ partials, TO* __restrict__ out,
+attention_scored_merge_kernel(const float* partials, TO* __restrict__ out,
                               const int* __restrict__ segment_of_token, const int* __restrict__ positions,
                               const float* __restrict__ sink, int n_values, int dv, int max_chunks, int num_segments,
-                              int window, int keep_first, int unnormalised, const float* __restrict__ out_gate) {
+                              int window, int keep_first, int unnormalised, const float* out_gate) {
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x, item = blockIdx.y, d = threadIdx.x;
@@ -324,8 +324,8 @@ template <> __device__ __forceinline__ void scored_store4<__nv_bfloat16>(__nv_bf
 
 // TW: the type of `wide` (float32, or bfloat16 from a kernel that writes its outputs rounded; then the rows are staged).
 template <typename TI, typename TO, typename TW>
-__global__ void head_mix_gate_kernel(const TW* __restrict__ wide, const float* __restrict__ mix,
-                                     const TI* __restrict__ gate_proj, int n_partials, long long partial_stride,
+__global__ void head_mix_gate_kernel(const TW* wide, const float* mix,
+                                     const TI* gate_proj, int n_partials, long long partial_stride,
                                      long long ld, const float* __restrict__ gate_bias,
                                      const int* __restrict__ segment_of_token, TO* __restrict__ out, int n_q, int n_kv,
                                      int n_values, int dv, int staged, int by_four) {

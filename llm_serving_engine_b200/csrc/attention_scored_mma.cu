@@ -40,15 +40,15 @@ template <int D> constexpr int tile_bytes(int rows) { return rows * (D * 2 + 16)
 
 template <int DK, int DV>
 __global__ void __launch_bounds__(128)
-attention_scored_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ kc,
-                            const __nv_bfloat16* __restrict__ vc, __nv_bfloat16* __restrict__ out,
+attention_scored_mma_kernel(const __nv_bfloat16* q, const __nv_bfloat16* kc,
+                            const __nv_bfloat16* vc, __nv_bfloat16* __restrict__ out,
                             float* __restrict__ out_f32, float* __restrict__ partials,
                             const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
-                            const int* __restrict__ segment_first_pos, int num_segments, const float* __restrict__ r1,
-                            const float* __restrict__ r2, const float* __restrict__ sink, int n_q, int n_kv,
+                            const int* __restrict__ segment_first_pos, int num_segments, const float* r1,
+                            const float* r2, const float* __restrict__ sink, int n_q, int n_kv,
                             int n_values, int page_size, float scale_log2e, int rows_per_tile, int num_pages,
                             int max_chunks, int window, int keep_first, float cap, const float* __restrict__ head_bias,
-                            const float* __restrict__ out_gate) {
+                            const float* out_gate) {
   constexpr int CHK = DK / 8, CHV = DV / 8;
   constexpr int K_BYTES = tile_bytes<DK>(BN), V_BYTES = tile_bytes<DV>(BN);
   extern __shared__ __align__(128) unsigned char smem[];

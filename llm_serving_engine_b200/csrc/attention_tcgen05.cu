@@ -104,9 +104,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ segment_start,
                        const int* __restrict__ segment_first_pos, int num_segments, int n_q, int n_kv, int page_size,
                        float scale_log2e, int num_pages, int skip_single, int parts, float* __restrict__ scratch,
-                       int* __restrict__ counters, const float* __restrict__ r1, const float* __restrict__ r2,
+                       int* __restrict__ counters, const float* r1, const float* r2,
                        const float* __restrict__ sink, int n_values, float cap,
-                       const float* __restrict__ out_gate) {
+                       const float* out_gate) {
   constexpr bool PEN = MODE == 1, SIG = MODE == 2;
   constexpr int HALVES = D / 64;
   constexpr uint32_t Q_BYTES = HALVES * HALF_BYTES, KV_BYTES = HALVES * HALF_BYTES, P_BYTES = 2 * HALF_BYTES;

@@ -46,7 +46,7 @@ template <> __device__ __forceinline__ void cn_store4<__nv_bfloat16>(__nv_bfloat
 // d and the sum: x (this thread's pieces threadIdx.x, threadIdx.x + blockDim.x, ... of four channels of one row) becomes
 // residual + d; returns the sum of squares over the row.  Every load is issued before any is used.
 template <typename TD, int C>
-__device__ __forceinline__ float cn_sum_row(const float* __restrict__ res, const TD* __restrict__ del, int n_partials,
+__device__ __forceinline__ float cn_sum_row(const float* res, const TD* del, int n_partials,
                                             long long partial_stride, const float* __restrict__ bias,
                                             const float* __restrict__ delta_weight, float delta_eps, int hidden,
                                             float* scratch, float (&x)[C][4]) {
@@ -119,7 +119,7 @@ __device__ __forceinline__ float cn_sum_row(const float* __restrict__ res, const
 // Every request brings one row: a block per row, which finds its predecessors in the window and moves it on.
 template <typename TD, typename TO, int TAPS, int C>
 __global__ void __launch_bounds__(512)
-conv_norm_single_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials, long long partial_stride,
+conv_norm_single_kernel(float* __restrict__ residual, const TD* delta, int n_partials, long long partial_stride,
                         const float* __restrict__ bias, const float* __restrict__ delta_weight, float delta_eps,
                         const float* __restrict__ weight, float eps, const float* __restrict__ conv_weight,
                         float* __restrict__ state, const int* __restrict__ segment_of_token,
@@ -197,7 +197,7 @@ conv_norm_single_kernel(float* __restrict__ residual, const TD* __restrict__ del
 // Many rows, first half: x in place, and every row's factor 1 / sqrt(mean(x^2) + eps).  A block per row.
 template <typename TD, int C>
 __global__ void __launch_bounds__(256)
-conv_norm_rows_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials, long long partial_stride,
+conv_norm_rows_kernel(float* __restrict__ residual, const TD* delta, int n_partials, long long partial_stride,
                       const float* __restrict__ bias, const float* __restrict__ delta_weight, float delta_eps, float eps,
                       float* __restrict__ factor, int hidden) {
   __shared__ float scratch[32];
@@ -223,8 +223,8 @@ conv_norm_rows_kernel(float* __restrict__ residual, const TD* __restrict__ delta
 constexpr int CN_ROWS = 16, CN_AHEAD = 4;
 template <typename TO, int TAPS>
 __global__ void __launch_bounds__(128)
-conv_norm_apply_kernel(const float* __restrict__ x, const float* __restrict__ factor, const float* __restrict__ weight,
-                       const float* __restrict__ conv_weight, const float* __restrict__ state,
+conv_norm_apply_kernel(const float* x, const float* factor, const float* __restrict__ weight,
+                       const float* __restrict__ conv_weight, const float* state,
                        const int* __restrict__ segment_of_token, const int* __restrict__ segment_start,
                        const int* __restrict__ segment_slot, TO* __restrict__ out, int tokens, int hidden, int num_slots,
                        int num_segments) {
@@ -308,7 +308,7 @@ conv_norm_apply_kernel(const float* __restrict__ x, const float* __restrict__ fa
 // The windows after a step of many rows: entry i holds h at the request's row count - (taps - 1) + i of this step, or moves up
 // from behind (in ascending order an entry only reads entries behind it).  grid (requests, channel tiles)
 __global__ void __launch_bounds__(128)
-conv_norm_state_kernel(const float* __restrict__ x, const float* __restrict__ factor, const float* __restrict__ weight,
+conv_norm_state_kernel(const float* x, const float* factor, const float* __restrict__ weight,
                        float* __restrict__ state, const int* __restrict__ segment_start,
                        const int* __restrict__ segment_slot, int hidden, int taps, int num_slots) {
   pdl_launch_dependents();
@@ -339,7 +339,7 @@ conv_norm_state_kernel(const float* __restrict__ x, const float* __restrict__ fa
 // A block per row; the row of x in shared memory.
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(256)
-delta_norm_rmsnorm_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+delta_norm_rmsnorm_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                           long long partial_stride, const float* __restrict__ bias,
                           const float* __restrict__ delta_weight, float delta_eps, const float* __restrict__ weight,
                           float eps, TO* __restrict__ out, const int* __restrict__ rows, int hidden, int tokens,
@@ -375,7 +375,7 @@ delta_norm_rmsnorm_kernel(float* __restrict__ residual, const TD* __restrict__ d
 // Four values a thread (by_four), else one.
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(256)
-residual_settle_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+residual_settle_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                        long long partial_stride, const float* __restrict__ bias, TO* __restrict__ copy, long long count,
                        int hidden, int by_four) {
   pdl_launch_dependents();
@@ -415,8 +415,8 @@ residual_settle_kernel(float* __restrict__ residual, const TD* __restrict__ delt
 
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(256)
-token_gate_kernel(const TI* __restrict__ z, int n_partials, long long partial_stride, long long ld,
-                  const TO* __restrict__ table, long long table_ld, int offset, const int* __restrict__ ids, int vocab,
+token_gate_kernel(const TI* z, int n_partials, long long partial_stride, long long ld,
+                  const TO* __restrict__ table, long long table_ld, int offset, const int* ids, int vocab,
                   TO* __restrict__ out, int tokens, int dim, int out_ld) {
   pdl_launch_dependents();
   pdl_wait();

@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(THREADS + 64, 1) decode_layers_kernel(const __
 // The rows' embeddings as the first layer's residual (packets of epoch 1) and what its norm reads; no epoch in every other packet,
 // UNSET in the other norms' places.
 __global__ void __launch_bounds__(256)
-decode_layers_start_kernel(const __nv_bfloat16* __restrict__ table, const int* __restrict__ ids, const float* __restrict__ norm,
+decode_layers_start_kernel(const __nv_bfloat16* __restrict__ table, const int* ids, const float* __restrict__ norm,
                            uint2* __restrict__ input, uint32_t* __restrict__ normed, uint4* __restrict__ rest, long long rest_count,
                            uint4* __restrict__ unset, long long unset_count, int rows, int hidden, int vocab, float scale) {
   pdl_launch_dependents();

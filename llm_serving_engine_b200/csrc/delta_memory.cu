@@ -115,7 +115,7 @@ __device__ __forceinline__ void dm_put(float* p, int lane, int width, const floa
 constexpr int DM_AHEAD = 4;
 template <typename TD, typename TO, int TAPS, bool VEC, int NS, bool ONE>
 __global__ void __launch_bounds__(128)
-delta_prepare_kernel(const TD* __restrict__ proj, int n_partials, long long partial_stride, long long ld,
+delta_prepare_kernel(const TD* proj, int n_partials, long long partial_stride, long long ld,
                      const float* __restrict__ conv_weight, float* __restrict__ state,
                      const int* __restrict__ segment_of_token, const int* __restrict__ segment_start,
                      const int* __restrict__ segment_slot, float* __restrict__ q_out, float* __restrict__ k_out,
@@ -281,8 +281,8 @@ constexpr int DS_ROWS = 32;        // rows of the state that a thread keeps
 // 32 rows of it in registers.  Requests of more than max_rows rows (max_rows > 0) are left to the chunked form.
 template <int PARTS>
 __global__ void __launch_bounds__(DS_THREADS)
-delta_scan_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
-                  const float* __restrict__ beta, const float* __restrict__ z, int z_partials, long long z_stride,
+delta_scan_kernel(const float* q, const float* k, const float* v,
+                  const float* beta, const float* z, int z_partials, long long z_stride,
                   long long z_ld, const float* __restrict__ dt_bias, const float* __restrict__ a_log,
                   float* __restrict__ state, const int* __restrict__ segment_start, const int* __restrict__ segment_slot,
                   float* __restrict__ out, int heads, int groups, int dim, int vdim, int num_slots, int max_rows) {

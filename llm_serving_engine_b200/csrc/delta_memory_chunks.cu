@@ -42,8 +42,8 @@ __host__ __device__ __forceinline__ long long dc_all(int dp, int ep) { return dc
 // of four channels; four rows a warp, so four warps.
 template <int NJ>
 __global__ void __launch_bounds__(128, 4)
-delta_chunk_prepare_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
-                           const float* __restrict__ beta, const float* __restrict__ z, int z_partials, long long z_stride,
+delta_chunk_prepare_kernel(const float* q, const float* k, const float* v,
+                           const float* beta, const float* z, int z_partials, long long z_stride,
                            long long z_ld, const float* __restrict__ dt_bias, const float* __restrict__ a_log,
                            const int* __restrict__ segment_start, float* __restrict__ buffer, int num_segments, int heads,
                            int groups, int dim, int vdim, int ep, int min_rows) {
@@ -211,7 +211,7 @@ __device__ __forceinline__ void dc_copy16(void* dst, const void* src) {
 // warps' sums [8][128] float4, u [16][16].
 template <int NJ>
 __global__ void __launch_bounds__(256)
-delta_chunk_scan_kernel(const float* __restrict__ buffer, float* __restrict__ state, const int* __restrict__ segment_start,
+delta_chunk_scan_kernel(const float* buffer, float* __restrict__ state, const int* __restrict__ segment_start,
                         const int* __restrict__ segment_slot, float* __restrict__ out, int heads, int dim, int vdim, int ep,
                         int num_slots, int min_rows) {
   constexpr int DP = 32 * NJ;

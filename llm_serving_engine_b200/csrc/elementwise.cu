@@ -16,7 +16,7 @@ LSE_CHECK_DEFINE(lse_check_elementwise)
 // ------------------------------------------------------------------ embedding
 // residual[t, :] = float(table[ids[t], :]) * scale; hidden_out (or null, one copy only) receives the same row rounded
 template <typename T>
-__global__ void embedding_kernel(const T* __restrict__ table, const int* __restrict__ ids,
+__global__ void embedding_kernel(const T* __restrict__ table, const int* ids,
                                  float* __restrict__ out, T* __restrict__ hidden_out, int hidden, int vocab, int copies,
                                  float scale) {
   LSE_TL_BEGIN(1)
@@ -74,7 +74,7 @@ extern "C" int lse_embedding(const void* table, int table_dtype, const int* ids,
 
 // out[t, :] += float(table[ids[t], :]) * scale      (rows with an id outside the table are left alone)
 template <typename T>
-__global__ void embedding_add_kernel(const T* __restrict__ table, const int* __restrict__ ids, float* __restrict__ out,
+__global__ void embedding_add_kernel(const T* __restrict__ table, const int* ids, float* __restrict__ out,
                                      int hidden, int vocab, float scale) {
   pdl_launch_dependents();
   pdl_wait();
@@ -134,7 +134,7 @@ constexpr int NORM_CHUNKS = 4;   // float4 chunks a thread keeps: hidden <= 512 
 // hidden % 4 == 0 and hidden <= NORM_THREADS * NORM_CHUNKS * 4.
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(NORM_THREADS)
-add_rmsnorm_vec_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+add_rmsnorm_vec_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                        long long partial_stride, const float* __restrict__ weight, TO* __restrict__ out,
                        const int* __restrict__ rows, int hidden, float eps, int write_residual, int source_rows) {
   LSE_TL_BEGIN(2)
@@ -206,7 +206,7 @@ add_rmsnorm_vec_kernel(float* __restrict__ residual, const TD* __restrict__ delt
 // sums a chunk cost the kernel above the rows in flight: 17 us for 1,349 rows of 3,584 (58 MB), against the 9 that the bytes take.
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(NORM_THREADS)
-add_rmsnorm_wide_kernel(float* __restrict__ residual, const TD* __restrict__ delta, const float* __restrict__ weight,
+add_rmsnorm_wide_kernel(float* __restrict__ residual, const TD* delta, const float* __restrict__ weight,
                         TO* __restrict__ out, int hidden, float eps) {
   pdl_launch_dependents();
   __shared__ float scratch[32];
@@ -253,7 +253,7 @@ add_rmsnorm_wide_kernel(float* __restrict__ residual, const TD* __restrict__ del
 
 // Any width: two passes over the row.
 template <typename TD, typename TO>
-__global__ void add_rmsnorm_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+__global__ void add_rmsnorm_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                                    long long partial_stride, const float* __restrict__ weight,
                                    TO* __restrict__ out, const int* __restrict__ rows, int hidden, float eps,
                                    int write_residual, int source_rows) {
@@ -297,7 +297,7 @@ __global__ void add_rmsnorm_kernel(float* __restrict__ residual, const TD* __res
 // hidden % 4 == 0, hidden <= 128 * C.
 template <typename TD, int C>
 __global__ void __launch_bounds__(256, C <= 12 ? 2 : 1)
-add_rmsnorm_rows_kernel(float* __restrict__ residual, const TD* __restrict__ delta, const float* __restrict__ weight,
+add_rmsnorm_rows_kernel(float* __restrict__ residual, const TD* delta, const float* __restrict__ weight,
                         __nv_bfloat16* __restrict__ out, int n_rows, int hidden, float eps) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -422,7 +422,7 @@ __device__ __forceinline__ void rope_rotate(float& xa, float& xb, float cs, floa
 template <typename T> __device__ __forceinline__ void rope_load4(const T* p, float (&v)[4]) { load4<T>(p, v); }
 
 template <typename TI, typename TO>
-__global__ void rope_kv_write_kernel(const TI* __restrict__ qkv, int n_partials, long long partial_stride,
+__global__ void rope_kv_write_kernel(const TI* qkv, int n_partials, long long partial_stride,
                                      const float* __restrict__ bias, const int* __restrict__ positions,
                                      const int* __restrict__ slot_mapping, const float* __restrict__ inv_freq,
                                      TO* __restrict__ q_out, TO* __restrict__ k_cache, TO* __restrict__ v_cache,
@@ -545,7 +545,7 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
 }
 
 template <typename TI, typename TO>
-__global__ void rope_kv_write_wide_kernel(const TI* __restrict__ qkv, const float* __restrict__ bias,
+__global__ void rope_kv_write_wide_kernel(const TI* qkv, const float* __restrict__ bias,
                                           const int* __restrict__ positions, const int* __restrict__ slot_mapping,
                                           const float* __restrict__ inv_freq, TO* __restrict__ q_out,
                                           TO* __restrict__ k_cache, TO* __restrict__ v_cache, int tokens, int n_q,
@@ -682,7 +682,7 @@ extern "C" int lse_rope_kv_write(const void* qkv, int in_dtype, int n_partials, 
 // gate_up[t] = [gate (I values) | up (I values)];  out[t, i] = silu(gate_i) * up_i
 // grid: (chunks of the row, tokens); a thread handles 4 consecutive i when I % 4 == 0.
 template <typename TI, typename TO, int VEC, int ACT>
-__global__ void silu_mul_kernel(const TI* __restrict__ gate_up, int n_partials, long long partial_stride,
+__global__ void silu_mul_kernel(const TI* gate_up, int n_partials, long long partial_stride,
                                 TO* __restrict__ out, int inter, float limit) {
   LSE_TL_BEGIN(4)
   pdl_launch_dependents();
@@ -723,7 +723,7 @@ __global__ void silu_mul_kernel(const TI* __restrict__ gate_up, int n_partials, 
 // numbered flat so that no block is half empty
 constexpr int SILU_UNROLL = 1;
 template <int ACT>
-__global__ void silu_mul_bf16x8_kernel(const __nv_bfloat16* __restrict__ gate_up, __nv_bfloat16* __restrict__ out,
+__global__ void silu_mul_bf16x8_kernel(const __nv_bfloat16* gate_up, __nv_bfloat16* __restrict__ out,
                                        int inter, long long total_chunks, float limit) {
   LSE_TL_BEGIN(4)
   pdl_launch_dependents();

@@ -56,7 +56,7 @@ __device__ __forceinline__ void halves(uint64_t v, float& lo, float& hi) {
 constexpr int BK = 16, STAGES = 4;
 template <int BM, int BN, int WM, int WN, int TM, int TN, bool IN_TMEM>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 32, IN_TMEM ? 2 : 1)
-gemm_f32_tiles_kernel(const float* __restrict__ A, const float* __restrict__ B, const float* __restrict__ bias,
+gemm_f32_tiles_kernel(const float* A, const float* __restrict__ B, const float* __restrict__ bias,
                       float* __restrict__ C, int M, int N, int K, long long lda, long long ldb, long long ldc,
                       long long part_stride) {
   constexpr int THREADS = (BM / WM) * (BN / WN) * 32, A_PITCH = BM + 4, B_PITCH = BN + 4;
@@ -237,7 +237,7 @@ constexpr int FEW_ROWS = 16;
 
 template <int ROWS, int TM, int TN, int GROUPS, int FEW_BK, int FEW_STAGES>
 __global__ void __launch_bounds__(32 * GROUPS * (ROWS / TM))
-gemm_f32_few_rows_kernel(const float* __restrict__ A, const float* __restrict__ B, const float* __restrict__ bias,
+gemm_f32_few_rows_kernel(const float* A, const float* __restrict__ B, const float* __restrict__ bias,
                          float* __restrict__ C, int M, int N, int K, long long lda, long long ldb, long long ldc,
                          long long part_stride, int stages) {
   constexpr int THREADS = 32 * GROUPS * (ROWS / TM), COLS = 32 * TN * GROUPS;

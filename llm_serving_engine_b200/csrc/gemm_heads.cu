@@ -11,9 +11,9 @@ constexpr int HG_TILE = 64, HG_K = 16, HG_THREADS = 256;
 
 template <typename TA, typename TW, typename TO>
 __global__ void __launch_bounds__(HG_THREADS)
-head_gemm_kernel(const TA* __restrict__ a, long long a_t, long long a_h, const TW* __restrict__ w, long long w_h,
+head_gemm_kernel(const TA* a, long long a_t, long long a_h, const TW* __restrict__ w, long long w_h,
                  long long w_k, long long w_n, TO* __restrict__ out, long long o_t, long long o_h,
-                 const float* __restrict__ gate, int gate_wide, int T, int N, int K) {
+                 const float* gate, int gate_wide, int T, int N, int K) {
   __shared__ float a_s[HG_K][HG_TILE + 4], w_s[HG_K][HG_TILE + 4];
   pdl_launch_dependents();
   pdl_wait();
@@ -92,9 +92,9 @@ template <> __device__ __forceinline__ void load_w8<__nv_bfloat16>(const __nv_bf
 // KSIDE: w_k == 1 and aligned for vector loads (grid.x = N / 16 columns a block); else grid.x = N / 32.
 template <typename TA, typename TW, typename TO, bool KSIDE>
 __global__ void __launch_bounds__(HF_THREADS)
-head_gemm_few_kernel(const TA* __restrict__ a, long long a_t, long long a_h, const TW* __restrict__ w, long long w_h,
+head_gemm_few_kernel(const TA* a, long long a_t, long long a_h, const TW* __restrict__ w, long long w_h,
                      long long w_k, long long w_n, TO* __restrict__ out, long long o_t, long long o_h,
-                     const float* __restrict__ gate, int gate_wide, int T, int N, int K) {
+                     const float* gate, int gate_wide, int T, int N, int K) {
   extern __shared__ __align__(16) float a_sh[];   // [HF_ROWS][K], then (columns side by side) [4][HF_ROWS][32] parts
   pdl_launch_dependents();
   pdl_wait();
@@ -188,7 +188,7 @@ head_gemm_few_kernel(const TA* __restrict__ a, long long a_t, long long a_h, con
 // A block per token, eight columns of one head a thread (by_eight) or one.
 template <typename TI>
 __global__ void __launch_bounds__(256)
-gate_heads_kernel(const TI* __restrict__ product, const TI* __restrict__ proj, long long ld, TI* __restrict__ out, int T, int heads,
+gate_heads_kernel(const TI* product, const TI* proj, long long ld, TI* __restrict__ out, int T, int heads,
                   int N, int by_eight) {
   pdl_launch_dependents();
   pdl_wait();

@@ -362,7 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(128 + 32 * FINISHERS
               if (c < here) {
                 float v = y[c];
                 if (scale != nullptr) {
-                  const float factor = __ldg(scale + at + c);
+                  const float factor = scale[at + c];
                   v = factor == 0.f ? 0.f : factor * v;
                 }
                 *dst = __float2bfloat16_rn(v);

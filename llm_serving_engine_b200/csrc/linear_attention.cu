@@ -22,7 +22,7 @@ namespace {
 // out[t] = o[t] / sqrt(mean(o[t]^2) + eps) * weight * sigmoid(g[t]); g: columns g_off .. g_off + n of proj.
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(256)
-gated_rmsnorm_kernel(const float* __restrict__ o, const TD* __restrict__ proj, int n_partials, long long partial_stride,
+gated_rmsnorm_kernel(const float* o, const TD* proj, int n_partials, long long partial_stride,
                      long long ld, int g_off, const float* __restrict__ weight, TO* __restrict__ out, int n, float eps,
                      const int* __restrict__ segment_of_token) {
   __shared__ float scratch[32];
@@ -45,7 +45,7 @@ gated_rmsnorm_kernel(const float* __restrict__ o, const TD* __restrict__ proj, i
 constexpr int GN_GROUPS = 4;
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(256)
-gated_rmsnorm_vec_kernel(const float* __restrict__ o, const TD* __restrict__ proj, long long ld, int g_off,
+gated_rmsnorm_vec_kernel(const float* o, const TD* proj, long long ld, int g_off,
                          const float* __restrict__ weight, TO* __restrict__ out, int n, float eps,
                          const int* __restrict__ segment_of_token) {
   __shared__ float scratch[32];
@@ -102,7 +102,7 @@ gated_rmsnorm_vec_kernel(const float* __restrict__ o, const TD* __restrict__ pro
 // keep = exp(-exp(a_log_h) dt), take = dt; z is column dt_off + h of proj.  A thread per (token, head).
 template <typename TD>
 __global__ void __launch_bounds__(256)
-ssd_gates_kernel(const TD* __restrict__ proj, int n_partials, long long partial_stride, long long ld, int dt_off,
+ssd_gates_kernel(const TD* proj, int n_partials, long long partial_stride, long long ld, int dt_off,
                  const float* __restrict__ dt_bias, const float* __restrict__ a_log, float* __restrict__ keep,
                  float* __restrict__ take, int tokens, int heads) {
   pdl_launch_dependents();
@@ -119,7 +119,7 @@ ssd_gates_kernel(const TD* __restrict__ proj, int n_partials, long long partial_
 // A decay per channel: keep = sigmoid(z + bias)^(1 / tau) = exp(log sigmoid(z + bias) / tau); z is column off + i of proj.
 template <typename TD>
 __global__ void __launch_bounds__(256)
-sigmoid_power_kernel(const TD* __restrict__ proj, int n_partials, long long partial_stride, long long ld, int off,
+sigmoid_power_kernel(const TD* proj, int n_partials, long long partial_stride, long long ld, int off,
                      const float* __restrict__ bias, float inv_tau, float* __restrict__ keep, int tokens, int n) {
   pdl_launch_dependents();
   pdl_wait();
@@ -141,8 +141,8 @@ sigmoid_power_kernel(const TD* __restrict__ proj, int n_partials, long long part
 constexpr int GGN_KEPT = 8;
 template <typename TD, typename TO, bool SINGLE>
 __global__ void __launch_bounds__(256)
-gated_group_rmsnorm_kernel(const float* __restrict__ o, const TD* __restrict__ proj, int n_partials,
-                           long long partial_stride, long long ld, int g_off, const TO* __restrict__ xsrc,
+gated_group_rmsnorm_kernel(const float* o, const TD* proj, int n_partials,
+                           long long partial_stride, long long ld, int g_off, const TO* xsrc,
                            long long x_ld, int x_off, const float* __restrict__ skip, int head_width,
                            const float* __restrict__ weight, int weight_len, TO* __restrict__ out, long long out_ld,
                            int n, int groups, float eps, float scale, int gate_first, int gate_act,
@@ -214,8 +214,8 @@ gated_group_rmsnorm_kernel(const float* __restrict__ o, const TD* __restrict__ p
 constexpr int GGN_WARP_KEPT = 16;
 template <typename TD, typename TO, bool SINGLE>
 __global__ void __launch_bounds__(256)
-gated_group_rmsnorm_warp_kernel(const float* __restrict__ o, const TD* __restrict__ proj, int n_partials,
-                                long long partial_stride, long long ld, int g_off, const TO* __restrict__ xsrc,
+gated_group_rmsnorm_warp_kernel(const float* o, const TD* proj, int n_partials,
+                                long long partial_stride, long long ld, int g_off, const TO* xsrc,
                                 long long x_ld, int x_off, const float* __restrict__ skip, int head_width,
                                 const float* __restrict__ weight, int weight_len, TO* __restrict__ out, long long out_ld,
                                 int tokens, int n, int groups, float eps, float scale, int gate_first, int gate_act,
@@ -394,7 +394,7 @@ __device__ __forceinline__ void lc_chunk(const int* __restrict__ segment_start, 
 // in shared memory as the product wants them, rows side by side, and neighbouring rows of the state come as pairs.
 template <typename TD>
 __global__ void __launch_bounds__(LC_THREADS, 2)
-linear_attention_own_states_kernel(const LcInput<TD> in, int k_off, int v_off, const float* __restrict__ decay,
+linear_attention_own_states_kernel(const LcInput<TD> in, int k_off, int v_off, const float* decay,
                                    const int* __restrict__ segment_start, float* __restrict__ chunk_state, int heads, int dim,
                                    int vdim, int num_segments) {
   extern __shared__ __align__(16) float smem[];
@@ -504,8 +504,8 @@ __device__ __forceinline__ void lc_product(uint64_t (&acc)[8][4], const float* a
 // while the other waits for its rows or its state.
 template <typename TD>
 __global__ void __launch_bounds__(LC_THREADS, 2)
-linear_attention_outputs_kernel(const LcInput<TD> in, int q_off, int k_off, int v_off, const float* __restrict__ decay,
-                                const int* __restrict__ segment_start, const float* __restrict__ chunk_state,
+linear_attention_outputs_kernel(const LcInput<TD> in, int q_off, int k_off, int v_off, const float* decay,
+                                const int* __restrict__ segment_start, const float* chunk_state,
                                 float* __restrict__ out, int heads, int dim, int vdim, int num_segments) {
   extern __shared__ __align__(16) float smem[];
   __shared__ float pow_s[LC_ROWS + 1];

@@ -42,13 +42,13 @@ __device__ __forceinline__ float la_act(float z, int act) { return act == 1 ? z 
 constexpr int MODE_PLAIN = 0, MODE_GATED = 1, MODE_VECTOR = 2;
 template <typename TD, int PARTS, bool OUTPUTS, int MODE>
 __global__ void __launch_bounds__(LA_THREADS, 4)     // four blocks an SM (measured faster than three blocks without the few spills)
-linear_attention_scan_kernel(const TD* __restrict__ proj, int n_partials, long long partial_stride, long long ld,
-                             int q_off, int k_off, int v_off, const float* __restrict__ decay,
+linear_attention_scan_kernel(const TD* proj, int n_partials, long long partial_stride, long long ld,
+                             int q_off, int k_off, int v_off, const float* decay,
                              float* __restrict__ state, const int* __restrict__ segment_start,
                              const int* __restrict__ segment_slot, float* __restrict__ out, int heads, int dim,
                              int vdim, int act, int num_slots, int num_segments, int chunk_rows, int phase,
-                             float* __restrict__ chunk_state, const float* __restrict__ token_keep,
-                             const float* __restrict__ token_take, float q_scale, int norm_col, int qk_share, int only_up_to) {
+                             float* __restrict__ chunk_state, const float* token_keep,
+                             const float* token_take, float q_scale, int norm_col, int qk_share, int only_up_to) {
   constexpr bool GATED = MODE == MODE_GATED;
   constexpr bool VECTOR = MODE == MODE_VECTOR;
   constexpr int CW = 32 / PARTS;
@@ -203,7 +203,7 @@ __device__ __forceinline__ int la_chunks(int rows, int chunk_rows, int short_row
 }
 template <int BATCH>
 __global__ void __launch_bounds__(256)
-linear_attention_carry_kernel(const float* __restrict__ decay, float* __restrict__ state,
+linear_attention_carry_kernel(const float* decay, float* __restrict__ state,
                               const int* __restrict__ segment_start, const int* __restrict__ segment_slot,
                               float* __restrict__ chunk_state, int heads, int dim, int vdim, int num_slots,
                               int chunk_rows, int short_rows) {
@@ -248,7 +248,7 @@ linear_attention_carry_kernel(const float* __restrict__ decay, float* __restrict
 // of one head's state of one request; its warps first multiply up every chunk's factors (shared memory, one number a
 // chunk), then every thread carries its element from chunk to chunk as above.  vs = columns of the state.
 __global__ void __launch_bounds__(256)
-linear_attention_gated_carry_kernel(const float* __restrict__ token_keep, float* __restrict__ state,
+linear_attention_gated_carry_kernel(const float* token_keep, float* __restrict__ state,
                                     const int* __restrict__ segment_start, const int* __restrict__ segment_slot,
                                     float* __restrict__ chunk_state, int heads, int dim, int vs, int num_slots,
                                     int chunk_rows) {
@@ -297,7 +297,7 @@ linear_attention_gated_carry_kernel(const float* __restrict__ token_keep, float*
 // The vector form's carry.  First every chunk's factors, one per row of the state: the product of its tokens' keep
 // vectors, chunk_keep[chunk][head][dim] (a block per chunk and head, a thread per row).
 __global__ void __launch_bounds__(256)
-linear_attention_chunk_keep_kernel(const float* __restrict__ token_keep, const int* __restrict__ segment_start,
+linear_attention_chunk_keep_kernel(const float* token_keep, const int* __restrict__ segment_start,
                                    float* __restrict__ chunk_keep, int heads, int dim, int num_segments, int chunk_rows) {
   pdl_launch_dependents();
   pdl_wait();
@@ -324,7 +324,7 @@ linear_attention_chunk_keep_kernel(const float* __restrict__ token_keep, const i
 
 // Then, as above, every element carried from chunk to chunk with its row's factor.
 __global__ void __launch_bounds__(256)
-linear_attention_vector_carry_kernel(const float* __restrict__ chunk_keep, float* __restrict__ state,
+linear_attention_vector_carry_kernel(const float* chunk_keep, float* __restrict__ state,
                                      const int* __restrict__ segment_start, const int* __restrict__ segment_slot,
                                      float* __restrict__ chunk_state, int heads, int dim, int vs, int num_slots,
                                      int chunk_rows) {
@@ -346,10 +346,20 @@ linear_attention_vector_carry_kernel(const float* __restrict__ chunk_keep, float
   float running = *slot;
   float* own = chunk_state + (size_t)before * per_state + at;
   const float* factor = chunk_keep + ((size_t)before * heads + h) * dim + d;
-  for (int c = 0; c < chunks; ++c) {
-    const float mine = own[(size_t)c * per_state];
-    own[(size_t)c * per_state] = running;
-    running = fmaf(factor[(size_t)c * heads * dim], running, mine);
+  for (int c0 = 0; c0 < chunks; c0 += 8) {
+    float mine[8], keep[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mine[i] = c0 + i < chunks ? own[(size_t)(c0 + i) * per_state] : 0.f;
+      keep[i] = c0 + i < chunks ? factor[(size_t)(c0 + i) * heads * dim] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c0 + i < chunks) {
+        own[(size_t)(c0 + i) * per_state] = running;
+        running = fmaf(keep[i], running, mine[i]);
+      }
+    }
   }
   *slot = running;
 }

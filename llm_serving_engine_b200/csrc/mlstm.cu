@@ -35,7 +35,7 @@ constexpr int MG_THREADS = 256;
 
 template <typename TD>
 __global__ void __launch_bounds__(MG_THREADS)
-mlstm_gates_kernel(const TD* __restrict__ proj, int n_partials, long long partial_stride, long long ld, int i_off,
+mlstm_gates_kernel(const TD* proj, int n_partials, long long partial_stride, long long ld, int i_off,
                    int f_off, const float* __restrict__ i_bias, const float* __restrict__ f_bias, float cap,
                    float* __restrict__ state_m, const int* __restrict__ segment_start,
                    const int* __restrict__ segment_slot, float* __restrict__ keep, float* __restrict__ take,
@@ -89,7 +89,7 @@ mlstm_gates_kernel(const TD* __restrict__ proj, int n_partials, long long partia
 // read [T, heads, vdim + 1]: the scan's outputs, the last column n . q.  A warp per (token, head).
 template <typename TD, typename TO>
 __global__ void __launch_bounds__(128)
-mlstm_readout_kernel(const float* __restrict__ read, const float* __restrict__ floor_in, const TD* __restrict__ proj,
+mlstm_readout_kernel(const float* read, const float* floor_in, const TD* proj,
                      int n_partials, long long partial_stride, long long ld, int g_off,
                      const float* __restrict__ weight, TO* __restrict__ out, int tokens, int heads, int vdim, float eps,
                      const int* __restrict__ segment_of_token) {

@@ -52,7 +52,7 @@ template <> __device__ __forceinline__ void rs_store<__nv_bfloat16>(__nv_bfloat1
 // VEC: channels a thread handles at a time (4: sixteen-byte loads and stores; H and the strides are multiples of 4).
 template <typename TD, typename TO, int VEC>
 __global__ void __launch_bounds__(RS_THREADS)
-streams_update_rmsnorm_kernel(float* __restrict__ X, const TD* __restrict__ delta, int n_partials,
+streams_update_rmsnorm_kernel(float* __restrict__ X, const TD* delta, int n_partials,
                               long long partial_stride, const float* __restrict__ scale, float mult,
                               const float* __restrict__ mix, const float* __restrict__ write_w,
                               const float* __restrict__ read_w, const float* __restrict__ weight,

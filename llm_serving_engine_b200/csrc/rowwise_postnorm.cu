@@ -39,7 +39,7 @@ template <> __device__ __forceinline__ void postnorm_store4<__nv_bfloat16>(__nv_
 // ------------------------------------------------------------------ embedding + learned positions
 template <typename T, typename TO>
 __global__ void embedding_positions_kernel(const T* __restrict__ table, const T* __restrict__ pos_table,
-                                           const int* __restrict__ ids, const int* __restrict__ positions, float scale,
+                                           const int* ids, const int* __restrict__ positions, float scale,
                                            float* __restrict__ residual, TO* __restrict__ hidden_out, int hidden,
                                            int vocab, int max_positions) {
   pdl_launch_dependents();
@@ -62,9 +62,9 @@ __global__ void embedding_positions_kernel(const T* __restrict__ table, const T*
 // (the compute-dtype copy of the residual; the residual itself when there is no copy);
 // residual <- y / sqrt(mean(y^2) + eps) * weight;  hidden_io <- the same, rounded.
 template <typename TD, typename TO>
-__global__ void scaled_add_rmsnorm_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+__global__ void scaled_add_rmsnorm_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                                           long long partial_stride, const float* __restrict__ bias,
-                                          const float* __restrict__ row_scale, float alpha,
+                                          const float* row_scale, float alpha,
                                           const float* __restrict__ weight, TO* __restrict__ hidden_io, int hidden,
                                           float eps) {
   pdl_launch_dependents();
@@ -101,9 +101,9 @@ __global__ void scaled_add_rmsnorm_kernel(float* __restrict__ residual, const TD
 // pair.  Few rows (decoding) wait for round trips, not for bandwidth: this form has three of them.
 template <typename TD, typename TO, int C>
 __global__ void __launch_bounds__(256)
-scaled_add_rmsnorm_regs_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials,
+scaled_add_rmsnorm_regs_kernel(float* __restrict__ residual, const TD* delta, int n_partials,
                                long long partial_stride, const float* __restrict__ bias,
-                               const float* __restrict__ row_scale, float alpha, const float* __restrict__ weight,
+                               const float* row_scale, float alpha, const float* __restrict__ weight,
                                TO* __restrict__ hidden_io, int hidden, float eps) {
   pdl_launch_dependents();
   pdl_wait();
@@ -187,7 +187,7 @@ scaled_add_rmsnorm_regs_kernel(float* __restrict__ residual, const TD* __restric
 // A warp owns one head of one token: items 0 .. n_q-1 are query heads, then n_kv key heads, then n_kv value heads.
 // The row of `proj` is [q (n_q * dk) | k (n_kv * dk) | v (n_kv * dv) | anything else].
 template <typename TI, typename TO>
-__global__ void head_norm_kv_write_kernel(const TI* __restrict__ proj, int n_partials, long long partial_stride,
+__global__ void head_norm_kv_write_kernel(const TI* proj, int n_partials, long long partial_stride,
                                           long long ld, const float* __restrict__ bias,
                                           const float* __restrict__ q_norm, const float* __restrict__ k_norm, float eps,
                                           const int* __restrict__ slot_mapping, TO* __restrict__ q_out,
@@ -293,13 +293,13 @@ __global__ void head_norm_kv_write_kernel(const TI* __restrict__ proj, int n_par
 // normed nor rotated).
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(128)
-head_norm_rope_kv_write_kernel(const TI* __restrict__ proj, int n_partials, long long partial_stride, long long ld,
+head_norm_rope_kv_write_kernel(const TI* proj, int n_partials, long long partial_stride, long long ld,
                                const float* __restrict__ bias, const float* __restrict__ q_norm,
                                const float* __restrict__ k_norm, float eps, const int* __restrict__ slot_mapping,
                                const int* __restrict__ positions, const double* __restrict__ freq, float rot_factor,
                                int rot_dims, TO* __restrict__ q_out, TO* __restrict__ k_cache, TO* __restrict__ v_cache,
                                int tokens, int n_q, int n_kv, int dk, int dv, int page_size, int num_pages,
-                               const float* __restrict__ q_factor, int values_are_keys) {
+                               const float* q_factor, int values_are_keys) {
   __shared__ float staged[4][256];
   pdl_launch_dependents();
   pdl_wait();
@@ -383,7 +383,7 @@ constexpr int PAIR_THREADS = 128, PAIR_MAX_WIDTH = 256;
 
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(PAIR_THREADS)
-head_norm_pair_rope_kernel(PairHeadArgs a, const TI* __restrict__ proj, TO* __restrict__ q_out, TO* __restrict__ k_cache,
+head_norm_pair_rope_kernel(PairHeadArgs a, const TI* proj, TO* __restrict__ q_out, TO* __restrict__ k_cache,
                            TO* __restrict__ v_cache) {
   __shared__ float cos_s[PAIR_MAX_WIDTH / 2], sin_s[PAIR_MAX_WIDTH / 2];
   pdl_launch_dependents();

@@ -31,7 +31,7 @@ __device__ __forceinline__ float uniform01(long long seed, long long counter) {
 }
 
 __global__ void __launch_bounds__(THREADS)
-argmax_kernel(const float* __restrict__ logits, long long row_stride, int vocab,
+argmax_kernel(const float* logits, long long row_stride, int vocab,
               int* __restrict__ out) {
   __shared__ float best_v[32];
   __shared__ int best_i[32];
@@ -89,7 +89,7 @@ constexpr int RADIX_BITS = 11;   // the bits of a value are decided 11, 11 and 1
 // bisection over the float's bits gave before).  Mass is counted in integers, 2^-31 of the whole mass `total` each
 // (32-bit sums, which do not depend on the order in which threads add: the threshold is the same in every run).
 // top_p = 0 keeps the largest values only.
-__device__ float top_p_threshold(const float* __restrict__ e, int vocab, float top_p, float total, unsigned* hist, int* chosen) {
+__device__ float top_p_threshold(const float* e, int vocab, float top_p, float total, unsigned* hist, int* chosen) {
   const float unit = 2147483648.0f / total;
   unsigned prefix = 0;              // the bits decided so far
   int done = 0;
@@ -174,7 +174,7 @@ __device__ float top_p_threshold(const float* __restrict__ e, int vocab, float t
 }
 
 __global__ void __launch_bounds__(THREADS)
-sample_kernel(const float* __restrict__ logits, long long row_stride, int vocab,
+sample_kernel(const float* logits, long long row_stride, int vocab,
               const float* __restrict__ temperature, const float* __restrict__ top_p,
               const long long* __restrict__ seed, const long long* __restrict__ counter,
               float* __restrict__ scratch, int* __restrict__ out) {

@@ -35,7 +35,7 @@ constexpr int SZ_TOKENS = 16, SZ_CHANNELS = 64, SZ_PARTS = 4;
 
 template <typename TD>
 __global__ void __launch_bounds__(SZ_CHANNELS * SZ_PARTS)
-ssm_step_sizes_kernel(const TD* __restrict__ low, int n_partials, long long partial_stride, long long ld,
+ssm_step_sizes_kernel(const TD* low, int n_partials, long long partial_stride, long long ld,
                       const float* __restrict__ weight_t, const float* __restrict__ bias, float* __restrict__ dt,
                       int tokens, int channels, int rank) {
   extern __shared__ float4 sz_smem[];     // [rank][16] inputs, then [3][16][64] sums of the parts after the first
@@ -95,9 +95,9 @@ ssm_step_sizes_kernel(const TD* __restrict__ low, int n_partials, long long part
 // B and C: columns b_off .. and c_off .. of `low`.
 template <typename TD, typename TL, typename TX, typename TO, int LANES>
 __global__ void __launch_bounds__(SS_THREADS)
-selective_scan_kernel(const TX* __restrict__ x, const float* __restrict__ dt, const TD* __restrict__ proj,
+selective_scan_kernel(const TX* x, const float* dt, const TD* proj,
                       int proj_partials, long long proj_stride, long long proj_ld, int z_off,
-                      const TL* __restrict__ low, int low_partials, long long low_stride, long long low_ld, int b_off,
+                      const TL* low, int low_partials, long long low_stride, long long low_ld, int b_off,
                       int c_off, const float* __restrict__ a_log, const float* __restrict__ skip,
                       float* __restrict__ state, const int* __restrict__ segment_start,
                       const int* __restrict__ segment_slot, TO* __restrict__ out, long long out_ld, float scale,
@@ -225,7 +225,7 @@ selective_scan_kernel(const TX* __restrict__ x, const float* __restrict__ dt, co
 __global__ void __launch_bounds__(256)
 selective_scan_carry_kernel(const float* __restrict__ a_log, float* __restrict__ state,
                             const int* __restrict__ segment_start, const int* __restrict__ segment_slot,
-                            float* __restrict__ chunk_state, const float* __restrict__ chunk_dt, int channels, int states,
+                            float* __restrict__ chunk_state, const float* chunk_dt, int channels, int states,
                             int num_slots, int chunk_rows) {
   pdl_launch_dependents();
   pdl_wait();

@@ -42,7 +42,7 @@ __device__ __forceinline__ void tn_store(T* p, const float (&v)[VEC]) {
 // loads in flight at a time.
 template <typename TD, typename TO, int VEC>
 __global__ void __launch_bounds__(256)
-tanh_norm_kernel(float* __restrict__ residual, const TD* __restrict__ delta, int n_partials, long long partial_stride,
+tanh_norm_kernel(float* __restrict__ residual, const TD* delta, int n_partials, long long partial_stride,
                  const float* __restrict__ after_alpha, const float* __restrict__ after_w,
                  const float* __restrict__ after_b, const float* __restrict__ before_alpha,
                  const float* __restrict__ before_w, const float* __restrict__ before_b, TO* __restrict__ out,
