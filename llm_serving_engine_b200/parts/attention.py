@@ -103,7 +103,8 @@ class GroupedQueryAttention(Mixer):
     def cache_requirement(cls, params, hidden_size):
         window, position = int(params.get("window", 0)), POSITION_ENCODINGS.get(params["position"]["kind"])
         return PagedKV(int(params["num_kv_heads"]), int(params["head_dim"]), window,
-                       int4=window == 0 and int(params["head_dim"]) in (64, 128) and position.int4)
+                       int4=(window == 0 and int(params["head_dim"]) in (64, 128) and getattr(position, "int4", False)
+                             and cls.forward is GroupedQueryAttention.forward))
 
     def prompt_kernel(self, segment_counts: list[int], page_size: int | None = None) -> str:
         """"tcgen05" or "mma": the kernel a step with prompt portions takes (the rule at the top of this file)."""

@@ -157,6 +157,11 @@ class Norm(Part):
 class PositionEncoding(Part):
     int4 = False           # whether encode_and_store also writes pages of 4 bits (cache.key_scales is not None)
 
+    def __init_subclass__(cls, **options) -> None:
+        super().__init_subclass__(**options)
+        if "encode_and_store" in vars(cls) and "int4" not in vars(cls):
+            cls.int4 = False       # (what a class says of its own encode_and_store says nothing of another's)
+
     def encode_and_store(self, qkv, bias, step, cache, q_out, n_q, n_kv, head_dim) -> None:
         raise NotImplementedError
 

@@ -59,3 +59,47 @@ def test_an_ordinary_launch_lies_between_a_steps_tables_and_its_kernels(monkeypa
         beam_search._Step(held, 0, False)._launch()
         at = order.index("step")
         assert {"own tables", "tables"} <= set(order[:at]) and order[at - 1] == "lengths" and "row lengths" in order[at:]
+
+
+def test_parts_of_their_own_are_not_given_pages_of_4_bits(monkeypatch):
+    """A rotation or an attention that replaces the one which knows 4-bit pages would write and read them as if they held bfloat16 numbers:
+    what was said of the other class does not hold for it."""
+    from llm_serving_engine_b200.cache.manager import CacheManager
+    from llm_serving_engine_b200.config import CacheConfig
+    from llm_serving_engine_b200.parts.attention import GroupedQueryAttention
+    from llm_serving_engine_b200.parts.base import POSITION_ENCODINGS, PositionEncoding
+    from llm_serving_engine_b200.parts.rope import RotaryEncoding
+
+    class Own(RotaryEncoding):
+        def encode_and_store(self, *args):
+            raise AssertionError
+
+    class OwnOf4Bits(RotaryEncoding):
+        int4 = True
+
+        def encode_and_store(self, *args):
+            raise AssertionError
+
+    class Named(RotaryEncoding):
+        pass
+
+    class Stranger:          # no PositionEncoding at all
+        pass
+
+    class OwnAttention(GroupedQueryAttention):
+        def forward(self, x, step, cache):
+            raise AssertionError
+
+    kinds = {"rope": RotaryEncoding, "own": Own, "own4": OwnOf4Bits, "named": Named, "stranger": Stranger, "wave": PositionEncoding}
+    monkeypatch.setattr(POSITION_ENCODINGS, "get", kinds.__getitem__)
+    for kind, taken in (("rope", True), ("own", False), ("own4", True), ("named", True), ("stranger", False), ("wave", False)):
+        params = {"num_heads": 4, "num_kv_heads": 2, "head_dim": 64, "position": {"kind": kind}}
+        for mixer, of_mixer in ((GroupedQueryAttention, True), (OwnAttention, False)):
+            need = mixer.cache_requirement(params, 256)
+            assert need.int4 == (taken and of_mixer), (kind, mixer)
+            CacheManager([need], CacheConfig(16, 4), torch.bfloat16, "cpu", 64)            # a bfloat16 cache in any case
+            if need.int4:
+                CacheManager([need], CacheConfig(16, 4, kv_bits=4), torch.bfloat16, "cpu", 64)
+            else:
+                with pytest.raises(ValueError, match="4 bits"):
+                    CacheManager([need], CacheConfig(16, 4, kv_bits=4), torch.bfloat16, "cpu", 64)
