@@ -278,6 +278,10 @@ class CacheManager:
         taken = [self._free_slots.popleft() for _ in range(slots)]
         request.lent = [had + new for had, new in zip(request.lent or [[] for _ in self.groups], lent)]
         request.lent_slots += taken
+        used = sum(group.pool.used_pages for group in self.groups)
+        if used >= self._high_water["blocks"]:
+            self._high_water["blocks"] = used
+            self._high_water_open = True
         return lent, taken
 
     def _extend(self, request: RequestCache, after: int) -> None:

@@ -103,3 +103,29 @@ def test_parts_of_their_own_are_not_given_pages_of_4_bits(monkeypatch):
             else:
                 with pytest.raises(ValueError, match="4 bits"):
                     CacheManager([need], CacheConfig(16, 4, kv_bits=4), torch.bfloat16, "cpu", 64)
+
+
+def test_lent_pages_count_in_the_most_that_were_used():
+    from llm_serving_engine_b200.cache.manager import CacheFullError, CacheManager
+    from llm_serving_engine_b200.config import CacheConfig
+    from llm_serving_engine_b200.parts.base import PagedKV
+
+    cache = CacheManager([PagedKV(2, 64), PagedKV(2, 128)], CacheConfig(16, 40), torch.float32, "cpu", 640, num_state_slots=4)
+    cache.create("a")
+    cache.reserve("a", 40)                       # three pages of either group
+    assert cache.grow("a", 30)                   # five
+    lent, slots = cache.lend("a", 6, 2)
+    assert [len(pages) for pages in lent] == [6, 6] and len(slots) == 2
+    with pytest.raises(CacheFullError):
+        cache.lend("a", 30, 0)
+    for _ in range(2):                           # while they are held, and afterwards
+        stats = cache.stats(contiguous_max_length=640)
+        assert stats["peak_blocks_used"] == 22 and stats["contiguous_waste_tokens"] == 640 - 40
+        if "a" in cache.requests:
+            assert stats["blocks_used"] == 22
+            cache.free("a")
+    assert cache.stats()["blocks_used"] == 0
+    cache.create("b")
+    cache.reserve("b", 16)
+    cache.lend("b", 1, 0)
+    assert cache.stats()["peak_blocks_used"] == 22
