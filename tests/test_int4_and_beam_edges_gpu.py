@@ -163,3 +163,55 @@ def test_portions_over_zeros():
         out = ops.paged_attention_prefill_int4(q, *some, torch.empty_like(q), tables, start, first, 0.125)
         assert portions(some, tables, counts, firsts, q, out, 0.125, 16) >= 6
         assert values or not out.any()
+
+
+# ------------------------------------------------------------------ the checked variant of the kernels
+CHECKED = r"""
+import random, sys
+sys.path.insert(0, {tests!r}); sys.path.insert(0, {root!r})
+import torch
+import helpers
+from test_beam_engine_gpu import engine_of, models
+from llm_serving_engine_b200 import GenerationConfig
+from llm_serving_engine_b200.engine import StepEntry
+from llm_serving_engine_b200.kernels import library
+
+model, rng = models(), random.Random(3)
+for page in (16, 8, 5):
+    engine = engine_of(model, page=page, pages=301, kv_bits=4)
+    engine.generate_many([helpers.random_tokens(rng, 512, n) for n in (3, 70, 130, 33)], GenerationConfig(max_new_tokens=12))
+    engine.beam_search([helpers.random_tokens(rng, 512, n) for n in (21, 37)], 5, 9, 7)
+    assert library.check_report() == [], library.check_report()
+for source in ("int4_cache", "attention_int4", "attention_int4_tcgen05", "beam_search", "step_tables"):
+    assert library.load().source_loaded(source), source
+print("clean: nothing recorded")
+
+# a table entry of -1 inside the context, made on the host: replaced and recorded by the kernels of portions and of rows
+for page, kernel in ((16, "attention_int4_tc"), (16, "attention_int4"), (5, "attention_int4_tc"), (5, "attention_int4")):
+    engine = engine_of(model, page=page, pages=100, kv_bits=4)
+    engine.runner.use_graphs = False
+    cache, tokens = engine.cache, helpers.random_tokens(rng, 512, 70)
+    cache.create("r")
+    engine.runner.run([StepEntry("r", tokens[:60], [])])
+    request = cache.requests["r"]
+    kept = request.tables[0][1]
+    request.tables[0][1] = request.tables_np[0][1] = -1
+    engine.runner.run([StepEntry("r", tokens[60:62] if kernel.endswith("tc") else tokens[60:61], [0])])
+    torch.cuda.synchronize()
+    report = library.check_report()
+    assert [line for line in report if line.startswith(kernel + ":")] and all("block-table entry -1" in line for line in report), report
+    request.tables[0][1] = request.tables_np[0][1] = kept
+    cache.free("r")
+    print("recorded:", report)
+"""
+
+
+def test_the_checked_kernels_of_the_4_bit_cache_record_nothing_on_good_steps_and_a_bad_table_entry():
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", CHECKED.format(tests=tests, root=os.path.dirname(tests))], env=dict(os.environ, LSE_CHECK="1"),
+                          capture_output=True, text=True, timeout=900)
+    assert done.returncode == 0, done.stdout[-3000:] + done.stderr[-3000:]
+    assert "clean: nothing recorded" in done.stdout and done.stdout.count("recorded:") == 4
