@@ -215,3 +215,82 @@ def test_the_checked_kernels_of_the_4_bit_cache_record_nothing_on_good_steps_and
                           capture_output=True, text=True, timeout=900)
     assert done.returncode == 0, done.stdout[-3000:] + done.stderr[-3000:]
     assert "clean: nothing recorded" in done.stdout and done.stdout.count("recorded:") == 4
+
+
+# ------------------------------------------------------------------ what a beam's cache holds
+def held_rows(cache, layer, table, length):
+    """Keys and values [length, heads, D] of a layer behind a block table, and the step of the codes (zero in bfloat16) [length, heads]."""
+    view, places = cache.layer_view(layer), torch.arange(length, device="cuda")
+    slots = (table[places // cache.page_size] * cache.page_size + places % cache.page_size).int()
+    if view.key_scales is None:
+        page, at = slots.long() // cache.page_size, slots.long() % cache.page_size
+        return [(t[page, :, at].double(), torch.zeros((length, t.shape[1]), device="cuda")) for t in (view.keys, view.values)]
+    k, v = (torch.empty((length, view.keys.shape[1], 2 * view.keys.shape[3]), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.kv_read_int4(view.keys, view.key_scales, view.values, view.value_scales, slots, k, v)
+    page, at = slots.long() // cache.page_size, slots.long() % cache.page_size
+    return [(k.double(), view.key_scales[page, :, at, 0].double()), (v.double(), view.value_scales[page, :, at, 0].double())]
+
+
+def same_rows(got, want) -> bool:
+    """Rows of two steps over the same tokens: numbers of a bfloat16 model within the suite's bound of what another batch gives (8 units of
+    2^-8 of the largest of a row); held in 4 bits, each off by half a step of its own row, and by what the rounded scale (15 steps of
+    2^-8) and centre (2^-8 of the number) move the range's ends; 2^-8 once more from reading back."""
+    for (a, step_a), (b, step_b) in zip(got, want):
+        most = torch.maximum(a.abs(), b.abs()).amax(-1, keepdim=True)
+        steps = torch.maximum(step_a, step_b)[..., None]
+        if not ((a - b).abs() <= (8 + 3) * 2.0 ** -8 * most + (1 + 2 * 15 * 2.0 ** -8) * steps).all():
+            return False
+    return True
+
+
+@pytest.mark.parametrize("kv_bits,page,beams,lengths", [(4, 16, 6, (37, 80)), (4, 5, 3, (21, 40)), (0, 16, 6, (37, 80)), (0, 16, 4, (30,))])
+def test_a_beams_pages_hold_the_keys_and_values_of_its_own_tokens(kv_bits, page, beams, lengths, monkeypatch):
+    """After any number of choices, pages shared, taken over and copied: layer by layer what one plain step over a beam's whole sequence
+    writes, and not what another beam's would."""
+    from llm_serving_engine_b200.engine import BeamSearch, StepEntry, beam_search
+    engine = engine_of(models(), page=page, pages=400, kv_bits=kv_bits)
+    steps = []
+
+    class Watched(beam_search._Step):
+        def __init__(self, *args):
+            super().__init__(*args)
+            self.chosen = []
+            steps.append(self)
+
+        def choose(self, logits):
+            out = super().choose(logits)
+            self.chosen.append(out.clone())
+            return out
+
+    monkeypatch.setattr(beam_search, "_Step", Watched)
+    rng = random.Random(7)
+    prompts = [helpers.random_tokens(rng, 512, n) for n in lengths]
+    for count in (2, 25):
+        for use_graph in (False, True):
+            BeamSearch(engine.runner, beams, 9, use_graph=use_graph).search(prompts, count)
+            watched = steps.pop()
+            held, told = watched.held, {}
+            fed = [part.tolist() for part in torch.stack(watched.chosen[:count - 1]).cpu()]      # the last choice was not run
+            told = {}
+            for request, prompt in enumerate(prompts):
+                for beam in range(beams):
+                    at, tokens = beam, []
+                    for chosen, parents in reversed(fed):
+                        tokens.append(chosen[request][at])
+                        at = parents[request][at]
+                    told[request, beam] = [*prompt, *reversed(tokens)]
+            assert held.row_lengths.tolist() == [len(told[key]) for key in sorted(told)]
+            tables = held.tables[0].clone()
+            kept = {key: [held_rows(engine.cache, layer, tables[key[0] * beams + key[1]], len(sequence)) for layer in range(3)] for key, sequence in told.items()}
+            plain_rows = {}
+            for key, sequence in told.items():
+                engine.cache.create("told")
+                engine.runner.run([StepEntry("told", sequence, [])])
+                table = torch.tensor(engine.cache.block_table(0, "told"), device="cuda")
+                plain_rows[key] = [held_rows(engine.cache, layer, table, len(sequence)) for layer in range(3)]
+                engine.cache.free("told")
+            for key, sequence in told.items():
+                assert all(same_rows(got, want) for got, want in zip(kept[key], plain_rows[key])), (key, count)
+                for other, another in told.items():
+                    if other[0] == key[0] and another != sequence:       # the bound tells one beam's rows from another's, in every layer
+                        assert not any(same_rows(got, want) for got, want in zip(kept[key], plain_rows[other])), (key, other)
