@@ -657,7 +657,9 @@ int launch_rows(const void* q, const Cache4& cache, void* out, float* scratch, c
                      (__nv_bfloat16*)out, part_o, part_ml, shares, block_tables, bt_stride, rows, tokens, n_q, scale * LOG2E,
                      group, gchunks, num_segments);
     if (err != cudaSuccess) return (int)err;
-    // more than eight parts a row on average: eight slices, so that the parts of one long row are added up by more than its few blocks
+    // More than eight parts a row on average: eight slices, so that the parts of one long row are added up by more than its few blocks.
+    // One slice and eight, us of both launches: a row of 28 / 4 heads over 30,000 keys (148 parts) 30.2 and 13.5, four of 12 / 2 over 8,000
+    // (74) 19.5 and 10.6, four of 40 / 8 over 8,000 (18) 18.1 and 17.4, sixteen of 8 heads of 64 over 6,000 (5) 21.5 and 23.2.
 #define LSE_INT4_COMBINE(SLICES)                                                                                                 \
   lse_launch(combine_runs_kernel<D, SLICES>, dim3((unsigned)tokens, (unsigned)columns, SLICES), dim3(COMBINE_THREADS), 0, stream,       \
              (const float4*)part_o, (const float2*)part_ml, (const int2*)shares, rows, (__nv_bfloat16*)out, n_q, group, gchunks)

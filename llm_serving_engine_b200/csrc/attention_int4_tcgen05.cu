@@ -25,13 +25,13 @@
 //                             beyond 2^14: float16 ends at 2^16).
 //   combine   with fewer blocks than SMs, several blocks share the keys of a tile; each leaves its part in a workspace of this
 //             call, and another launch adds them up, in the order of the parts.
-// What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 294 us, 1.02 PFLOP/s (324 at the power cap): tensor
+// What bounds attend: 2,048 rows behind 6,144 keys, 40 / 8 heads of 128 (301 GFLOP) take 297 us, 1.01 PFLOP/s (327 to 342 at the power cap): tensor
 // cores busy for 58% of the cycles, the unit of the exponentials for 58% (128 x 128 a tile at 16 a cycle), and 656 blocks leave a
-// fifth turn of the SMs half empty.  Side by side, 324: all exponentials of a tile before the wait for the product of the tile
+// fifth turn of the SMs half empty.  Side by side with 324 (before the scales were measured, 3 us): all exponentials of a tile before the wait for the product of the tile
 // before 350, a quarter of them 338; a quarter of the exponentials by a polynomial 361; scores read twice from tensor memory, 32 at a
 // time, 354.  Small launches: a block's way from its start to its first scores (2.7 us), through a few tiles and to its end is 8 us,
-// and eight portions of about 200 rows (160 blocks, 24.1 us) make some SMs go it twice; starting the blocks with most keys first
-// took 26.6 (the search for them costs every block more than the order wins).
+// and eight portions of about 200 rows (160 blocks, 25.6 us) make some SMs go it twice; starting the blocks with most keys first
+// took 26.6 instead of 24.1 (the search for them costs every block more than the order wins).
 // Every wait is bounded (see tcgen05.cuh); a block whose wait gave up leaves NaN in its rows, frees its tensor memory and returns.
 #include <cuda_fp16.h>
 
@@ -47,6 +47,8 @@ constexpr int BM = 128, BN = 128, GROUPS = 2, GROUP_THREADS = 128;
 constexpr int MMA_WARP = 8, LOADER_WARP = 9, PV_WARP = 10, THREADS = 352;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f, REDO_STEP = 14.0f;   // in powers of two
+// (two portions of 128 rows behind 2,000 keys of 12 / 2 heads, six parts: 21.2 us; two tiles a part 27.0, eight 23.8; a portion of 16 rows
+// behind 30,000 keys of 28 / 4 heads, one part 240, two 139, four 86, eight 62)
 constexpr int MIN_TILES_A_PART = 4, MAX_PARTS = 8;
 constexpr uint32_t HALF_BYTES = 128 * 128;                // 128 rows x 64 float16
 constexpr float MOST_KEY = 65504.0f * 256.0f, MOST_VALUE = 65504.0f;       // rows beyond become NaN

@@ -8,8 +8,10 @@
 // Two launches.  chunk: a warp takes a piece of a beam's row, once from memory into registers, and leaves its maximum and its sum of
 // exponentials, a block its K best logits (only these can be among the request's K best).  Candidates are found without a sort: of the
 // lanes' 32 maxima the K-th largest is a bound that at least K values reach, and hardly more than K do.
-// merge: a block per request, from the chunks' leavings.  Offers are compared in 64 bits: two beams' offers can be closer than
-// float32 tells apart, and lse's error would decide.
+// merge: a block per request, from the chunks' leavings.  Warps' sums are added up, and offers made and compared, in 64 bits: two beams'
+// offers can be closer than float32 tells apart.  A warp's own sum is float32 (a logit's exponential is off by |logit - maximum| 2^-22
+// and the approximation's 2^-22, the 64 additions a lane by 2^-24 each), so a row's lse is off by 2^-22 as a rule, and two beams'
+// offers that are closer than that may come in either order; offers of one beam share its lse, and may not.
 // What bounds the choice: the logits are read once, 4 bytes each.  256 rows of 151,936 (32 requests of 8 beams, 156 MB) take 36 us for
 // both launches, 4.3 TB/s: the second turn of the SMs' blocks ends unevenly, and merge is 4 us; 4 rows 8.9 us, most of it the two
 // launches' latencies.  Pieces of twice the length 37 to 40 us, one more block an SM 38, loads past the L1 44.
@@ -22,10 +24,11 @@
 namespace {
 
 constexpr int MAX_BEAMS = 32;
+constexpr int SMS = 148;             // of a B200, which all this is compiled for
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Best { float value; int token; };
-struct Sum { double sum; float maximum, unused; };      // of a chunk: its exponentials add up to sum exp(maximum)
+struct Sum { double sum; float maximum; };      // of a chunk: its exponentials add up to sum exp(maximum)
 
 constexpr int CHUNK_WARPS = 4, GROUPS = 32;
 constexpr int LIST = 512;          // candidates above the bound that merge has room for (ties can make them any number)
@@ -206,7 +209,7 @@ beam_chunk_kernel(const float* logits, long long row_stride, int vocab, int beam
     if (m != -INFINITY && m != highest) s *= exp((double)m - (double)highest);
 #pragma unroll
     for (int o = CHUNK_WARPS / 2; o > 0; o >>= 1) s += shfl_xor_double(s, o);
-    if (lane == 0) sums[(size_t)row * chunks + chunk] = {s, highest, 0.f};
+    if (lane == 0) sums[(size_t)row * chunks + chunk] = {s, highest};
   }
   // The block's best: one's rank is its place in its own warp's list and how far it comes in the others', which are in order too.
   Best* out = best + ((size_t)row * chunks + chunk) * beams;
@@ -448,10 +451,10 @@ beam_reorder_kernel(const int* parents, int beams, const int* tables, int table_
 }
 
 int steps_of(long long rows, int vocab) {
-  // the largest pieces that leave a block for each of 148 SMs, or the smallest (4 rows of 151,936 values: 8.3 us with two steps, 9.5 with
+  // the largest pieces that leave a block for each SM, or the smallest (4 rows of 151,936 values: 8.3 us with two steps, 9.5 with
   // one; 120 of 100,001: 19.7 with eight, 21.9 with two)
   int steps = 8;
-  while (steps > 1 && rows * vocab < 148LL * CHUNK_WARPS * steps * STEP * 32) steps /= 2;
+  while (steps > 1 && rows * vocab < (long long)SMS * CHUNK_WARPS * steps * STEP * 32) steps /= 2;
   return steps;
 }
 int chunks_of(long long rows, int vocab) {
@@ -532,7 +535,7 @@ extern "C" int lse_beam_reorder(const int* parents, int requests, int beams, con
   }
   const long long rows = (long long)requests * beams;
   // about eight blocks an SM, two thirds of which find nothing to copy (a child that goes on in its parent's page)
-  const long long slices = rows < 8 * 148 ? 8 * 148 / rows : 1;
+  const long long slices = rows < 8 * SMS ? 8 * SMS / rows : 1;
   const dim3 grid((unsigned)rows, (unsigned)(most > slices ? slices : most));
 #define LSE_REORDER(V) lse_launch(beam_reorder_kernel<V>, grid, dim3(256), 0, stream, parents, beams, tables, table_stride, width, lengths, \
                                   page_size, new_tables, new_stride, list)

@@ -2342,7 +2342,11 @@ def paged_attention_prefill_int4(q: torch.Tensor, k_codes: torch.Tensor, k_scale
     a_head = capacity * INT4_TILE * dim
     heads_at_once = min(n_kv, max(1, INT4_WORKSPACE_BYTES // (4 * a_head)))
     with_tiles = min(segments, max_portions) if skip_single and max_portions > 0 else segments
-    # several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs
+    # Several blocks share a tile's keys while the launch has fewer blocks than the GPU has SMs.  With 8 blocks (16 rows of 28 / 4 heads
+    # behind 30,000 keys) one part takes 240 us, the rule's eight 62; with 36 (128 behind 8,000) 70 alone, 34 with four, 45 with six (the
+    # rule: five); with 32 (64 of 40 / 8 behind 4,000) 42 alone, 24 with six, 32 with eight (five); with 80 (two of 100 of 40 / 8 behind
+    # 2,000) 29.5 alone, 27.9 with two (two), 36 with three; with 100 (two of 200 of 28 / 4 behind 2,000) 28.8 alone (one), 39 with two.
+    # Short contexts lose the second launch: four of 100 of 12 / 2 behind 500 keys 14.0 alone, 17.4 with the rule's three.
     blocks = (-(-tokens // (INT4_TILE // group)) + with_tiles) * heads_at_once
     parts = max(1, min(8, 5 * sm_count() // (4 * blocks)))
     # float16 keys, values and queries, the powers of two in them, and (several parts) float32 outputs, maxima and sums of every part
