@@ -45,8 +45,9 @@ class BeamSearch:
         self.use_graph = runner.use_graphs if use_graph is None else use_graph
 
     def search(self, prompts: list[list[int]], max_new_tokens: int) -> list[list[Beam]]:
-        """The best ``beams`` continuations of every prompt, the best first (fewer where the model's logits leave fewer).  Raises
-        ``KernelError`` when a kernel's bounded wait gave up meanwhile, or no beam of a prompt is left."""
+        """The best ``beams`` continuations of every prompt, the best first (fewer where the model's logits leave fewer).
+        Pages for ``max_new_tokens`` of every beam, and a state slot a beam, are taken before the first choice: ``CacheFullError`` where
+        they are not free.  Raises ``KernelError`` when a kernel's bounded wait gave up meanwhile, or no beam of a prompt is left."""
         runner, cache = self.runner, self.runner.cache
         if not prompts or max_new_tokens <= 0:
             raise ValueError("a search needs prompts and a positive max_new_tokens")
